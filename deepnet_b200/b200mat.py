@@ -122,6 +122,11 @@ def _check(err_code):
         raise generate_exception(err_code)
 
 
+def _p(mat):
+    """The handle of a matrix that may be left out."""
+    return mat.p_mat if mat is not None else None
+
+
 _device_checked = False
 
 
@@ -299,6 +304,16 @@ class CUDAMatrix(object):
         _check(_lib.dropout(CUDAMatrix.rnd_state_p, self.p_mat, ct.c_float(dropprob), ct.c_float(val)))
         return self
 
+    def dropout_scaled(self, dropprob, target=None, add=None, key=None):
+        """target = add + (kept ? self / (1 - dropprob) : 0): dropout whose mean is self, joined to a residual.  No mask is stored;
+        returns the key (seed, call) that draws it.  With `key` the mask of an earlier call is drawn again (its gradient:
+        `dy.dropout_scaled(dropprob, key=key)`) and the random state stays as it is; without, a sampling call is consumed."""
+        target = target or self
+        state = CUDAMatrix.rnd_state if key is None else rnd_struct(*key)
+        key = (state.seed, state.calls)
+        _check(_lib.dropout_scaled(ct.byref(state), self.p_mat, _p(add), target.p_mat, ct.c_float(dropprob)))
+        return key
+
     # -- broadcasts --------------------------------------------------------
     def _vec_op(self, fn, vec, target, *extra):
         target = target or self
@@ -388,6 +403,38 @@ class CUDAMatrix(object):
         """cudamat/cudamat.py:1000-1016: columns longer than `norm` are scaled back to it (axis 0 only)."""
         target = target or self
         _check(_lib.normlimit_by_axis(self.p_mat, target.p_mat, ct.c_int(axis), ct.c_float(norm)))
+        return target
+
+    def layer_norm(self, gain=None, bias=None, eps=1e-5, target=None, stats=None):
+        """target[:, j] = gain * (self[:, j] - mean) / sqrt(variance + eps) + bias, every column by its own mean and variance.
+        stats (2 x columns, optional) receives what `layer_norm_deriv` needs; then self has to stay as it is until that call."""
+        target = target or self
+        _check(_lib.layer_norm(self.p_mat, _p(gain), _p(bias), target.p_mat, _p(stats), ct.c_float(eps)))
+        return target
+
+    def layer_norm_deriv(self, mat, stats, gain=None, target=None, grad_gain=None, grad_bias=None):
+        """self is the gradient of `mat.layer_norm(gain, bias, ..., stats=stats)`; target (default self) = the gradient of mat, grad_gain
+        and grad_bias (optional, one value a row) = those of gain and bias."""
+        target = target or self
+        _check(_lib.layer_norm_deriv(self.p_mat, mat.p_mat, stats.p_mat, _p(gain), target.p_mat, _p(grad_gain), _p(grad_bias)))
+        return target
+
+    def log_prob(self, tokens=None, target=None, entropy=None, stats=None, top=None, top_tokens=None):
+        """target (1 x columns) = log softmax(self[:, j])[tokens[j]] (tokens: float32 row of whole numbers; negative ones count from the
+        end, one out of range gives NaN).  Optional outputs: entropy (1 x columns) of each column's distribution, top and
+        top_tokens (k x columns, k <= 32): the k likeliest tokens' log probabilities and numbers, likeliest first, of equal logits the
+        lower number; stats (2 x columns), which `log_prob_deriv` needs.  Returns target (None without tokens)."""
+        if target is None and tokens is not None:
+            target = empty((1, self.shape[1]))
+        _check(_lib.log_prob(self.p_mat, _p(tokens), _p(target), _p(entropy), _p(stats), _p(top), _p(top_tokens)))
+        return target
+
+    def log_prob_deriv(self, tokens, stats, grad, entropy=None, grad_entropy=None, target=None):
+        """self are logits that `log_prob` was called on with these tokens; target (default self) = their gradient, from grad (1 x
+        columns), the gradient of the log probabilities, and grad_entropy, that of the entropies (with `entropy` as log_prob gave
+        them).  Columns whose gradients are 0 give 0 and are not read."""
+        target = target or self
+        _check(_lib.log_prob_deriv(self.p_mat, _p(tokens), stats.p_mat, _p(grad), _p(entropy), _p(grad_entropy), target.p_mat))
         return target
 
     def transpose(self, target=None):

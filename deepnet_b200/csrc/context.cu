@@ -218,6 +218,24 @@ void* workspace_zeroed(int slot, size_t bytes) {
   return p;
 }
 
+CallScratch::CallScratch(int slot, size_t bytes) : p(nullptr), of_graph(false) {
+  if (bytes == 0) return;
+  if (!stream_capturing()) {
+    p = workspace(slot, bytes);
+    return;
+  }
+  if (bytes > g_scratch_limit || cudaMallocAsync(&p, bytes, stream()) != cudaSuccess) {
+    cudaGetLastError();
+    p = nullptr;
+    set_error("workspace allocation failed");
+    return;
+  }
+  of_graph = true;
+}
+CallScratch::~CallScratch() {
+  if (of_graph && cudaFreeAsync(p, stream()) != cudaSuccess) set_error(cudaGetErrorString(cudaGetLastError()));
+}
+
 }  // namespace b200
 
 using namespace b200;

@@ -1,0 +1,425 @@
+// Layer normalisation of columns (one case a column) and its derivative.
+//   m = mean(x), r = 1 / sqrt(mean((x - m)^2) + eps), xh = (x - m) r, y = gain xh + bias
+//   a = gain dy:  dx = r (a - mean(a) - xh mean(a xh)),  dgain = sum over columns of dy xh,  dbias = sum over columns of dy
+// Bound by HBM: 8 bytes an element forward, 12 back.  A column is read once into registers (the variance is that of the
+// centred values), by a warp up to 1024 rows (256 where rows are not whole groups of four), by a block beyond.  Back, a block
+// walks columns and keeps its share of both parameters' gradients in registers; the blocks' shares are added by a second
+// launch in a fixed order, so results do not change from run to run.
+#include "common.cuh"
+
+using namespace b200;
+
+namespace {
+
+constexpr int kWarpsPerBlock = 8;        // columns a block works on side by side where a warp holds one
+
+// Sum over the threads of a column: the warp, or with `block` the whole block (red: 32 floats, free again on return
+// of the next call but one: the callers alternate between two).
+template <bool kBlock>
+__device__ __forceinline__ float column_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (kBlock) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    if (lane == 0) red[wid] = v;
+    __syncthreads();
+    v = lane < nw ? red[lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
+  return v;
+}
+// Both sums of a pair, with one barrier.
+template <bool kBlock>
+__device__ __forceinline__ float2 column_sum2(float2 v, float2* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  if (kBlock) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    if (lane == 0) red[wid] = v;
+    __syncthreads();
+    v = lane < nw ? red[lane] : make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+  }
+  return v;
+}
+
+// kVec consecutive floats (4: the address is on 16 bytes).
+template <int kVec>
+__device__ __forceinline__ void load(const float* p, float (&v)[kVec]) {
+  if constexpr (kVec == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  } else {
+    v[0] = *p;
+  }
+}
+template <int kVec>
+__device__ __forceinline__ void store(float* p, const float (&v)[kVec]) {
+  if constexpr (kVec == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else *p = v[0];
+}
+
+// kPer groups of kVec values a thread; h / kVec <= kPer * threads of a column.
+template <int kVec, int kPer, bool kBlock>
+__global__ void __launch_bounds__(kBlock ? 1024 : 32 * kWarpsPerBlock)
+    k_layer_norm(const float* x, const float* gain, const float* bias, float* y, float* stats, int h, int w, float eps) {
+  __shared__ float red[2][32];
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int threads = kBlock ? blockDim.x : 32, t = kBlock ? threadIdx.x : threadIdx.x & 31;
+  const int c = kBlock ? blockIdx.x : blockIdx.x * kWarpsPerBlock + (threadIdx.x >> 5);
+  if (c >= w) return;
+  const float* col = x + (long)c * h;
+  float v[kPer][kVec], s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    const int r = kVec * (t + i * threads);
+    if (r < h) {
+      load<kVec>(col + r, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; j++) v[i][j] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; i++)
+#pragma unroll
+    for (int j = 0; j < kVec; j++) s += v[i][j];
+  const float m = column_sum<kBlock>(s, red[0]) / h;
+  s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPer; i++)
+    if (kVec * (t + i * threads) < h) {
+#pragma unroll
+      for (int j = 0; j < kVec; j++) s += (v[i][j] - m) * (v[i][j] - m);
+    }
+  const float rs = 1.0f / sqrtf(column_sum<kBlock>(s, red[1]) / h + eps);
+  float* out = y + (long)c * h;
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    const int r = kVec * (t + i * threads);
+    if (r >= h) continue;
+    float g[kVec], b[kVec];
+    if (gain) load<kVec>(gain + r, g);
+    if (bias) load<kVec>(bias + r, b);
+#pragma unroll
+    for (int j = 0; j < kVec; j++) {
+      float xh = (v[i][j] - m) * rs;
+      if (gain) xh *= g[j];
+      v[i][j] = bias ? xh + b[j] : xh;
+    }
+    store<kVec>(out + r, v[i]);
+  }
+  if (stats && t == 0) {
+    stats[2L * c] = m;
+    stats[2L * c + 1] = rs;
+  }
+}
+
+// Columns too long for registers: one block a column, which reads it three times (twice from L2).
+__global__ void __launch_bounds__(1024) k_layer_norm_long(const float* x, const float* gain, const float* bias, float* y, float* stats,
+                                                          int h, int w, float eps) {
+  __shared__ float red[2][32];
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int c = blockIdx.x;
+  const float* col = x + (long)c * h;
+  float* out = y + (long)c * h;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int r = threadIdx.x; r < h; r += blockDim.x) s += col[r];
+  const float m = column_sum<true>(s, red[0]) / h;
+  s = 0.0f;
+#pragma unroll 8
+  for (int r = threadIdx.x; r < h; r += blockDim.x) s += (col[r] - m) * (col[r] - m);
+  const float rs = 1.0f / sqrtf(column_sum<true>(s, red[1]) / h + eps);
+#pragma unroll 4
+  for (int r = threadIdx.x; r < h; r += blockDim.x) {
+    float xh = (col[r] - m) * rs;
+    if (gain) xh *= gain[r];
+    out[r] = bias ? xh + bias[r] : xh;
+  }
+  if (stats && threadIdx.x == 0) {
+    stats[2L * c] = m;
+    stats[2L * c + 1] = rs;
+  }
+}
+
+// Back.  part: blocks x 2 x h, this block's sums of dy xh and of dy (or null: no parameter's gradient is wanted).
+template <int kVec, int kPer, bool kBlock>
+__global__ void __launch_bounds__(kBlock ? 512 : 32 * kWarpsPerBlock)
+    k_layer_norm_deriv(const float* dy, const float* x, const float* stats, const float* gain, float* dx, float* part, int h, int w) {
+  extern __shared__ float shares[];
+  __shared__ float2 red[2][32];
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int threads = kBlock ? blockDim.x : 32, t = kBlock ? threadIdx.x : threadIdx.x & 31;
+  const int first = kBlock ? blockIdx.x : blockIdx.x * kWarpsPerBlock + (threadIdx.x >> 5);
+  const int step = kBlock ? gridDim.x : gridDim.x * kWarpsPerBlock;
+  const float inv = 1.0f / h;
+  float dg[kPer][kVec], db[kPer][kVec];
+#pragma unroll
+  for (int i = 0; i < kPer; i++)
+#pragma unroll
+    for (int j = 0; j < kVec; j++) dg[i][j] = db[i][j] = 0.0f;
+  int turn = 0;
+  for (long c = first; c < w; c += step, turn ^= 1) {
+    const float m = stats[2 * c], rs = stats[2 * c + 1];
+    float v[kPer][kVec], d[kPer][kVec];
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const int r = kVec * (t + i * threads);
+      if (r < h) {
+        load<kVec>(x + c * h + r, v[i]);
+        load<kVec>(dy + c * h + r, d[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; j++) v[i][j] = m, d[i][j] = 0.0f;
+      }
+    }
+    float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const int r = kVec * (t + i * threads);
+      float g[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; j++) g[j] = 1.0f;
+      if (gain && r < h) load<kVec>(gain + r, g);
+#pragma unroll
+      for (int j = 0; j < kVec; j++) {
+        const float xh = (v[i][j] - m) * rs;
+        v[i][j] = xh;
+        dg[i][j] += d[i][j] * xh;
+        db[i][j] += d[i][j];
+        d[i][j] *= g[j];
+        s.x += d[i][j];
+        s.y += d[i][j] * xh;
+      }
+    }
+    s = column_sum2<kBlock>(s, red[turn]);
+    const float ma = s.x * inv, mx = s.y * inv;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const int r = kVec * (t + i * threads);
+      if (r >= h) continue;
+#pragma unroll
+      for (int j = 0; j < kVec; j++) d[i][j] = rs * (d[i][j] - ma - v[i][j] * mx);
+      store<kVec>(dx + c * h + r, d[i]);
+    }
+  }
+  if (!part) return;
+  float* out = part + 2L * blockIdx.x * h;
+  if (kBlock) {
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const int r = kVec * (t + i * threads);
+      if (r >= h) continue;
+      store<kVec>(out + r, dg[i]);
+      store<kVec>(out + h + r, db[i]);
+    }
+    return;
+  }
+  // the block's warps one after another
+  for (int k = 0; k < kWarpsPerBlock; k++) {
+    if ((threadIdx.x >> 5) == k) {
+#pragma unroll
+      for (int i = 0; i < kPer; i++)
+#pragma unroll
+        for (int j = 0; j < kVec; j++) {
+          const int r = kVec * (t + i * threads) + j;
+          if (r >= h) continue;
+          shares[r] = k ? shares[r] + dg[i][j] : dg[i][j];
+          shares[h + r] = k ? shares[h + r] + db[i][j] : db[i][j];
+        }
+    }
+    __syncthreads();
+  }
+  for (int r = threadIdx.x; r < 2 * h; r += blockDim.x) out[r] = shares[r];
+}
+
+// Long columns: dx as above with the columns read twice, and the shares of the parameters' gradients by rows.
+__global__ void __launch_bounds__(1024) k_layer_norm_deriv_long(const float* dy, const float* x, const float* stats, const float* gain,
+                                                                float* dx, int h, int w) {
+  __shared__ float2 red[32];
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const long c = blockIdx.x;
+  const float m = stats[2 * c], rs = stats[2 * c + 1], inv = 1.0f / h;
+  float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+  for (int r = threadIdx.x; r < h; r += blockDim.x) {
+    const float a = dy[c * h + r] * (gain ? gain[r] : 1.0f);
+    s.x += a;
+    s.y += a * ((x[c * h + r] - m) * rs);
+  }
+  s = column_sum2<true>(s, red);
+  const float ma = s.x * inv, mx = s.y * inv;
+#pragma unroll 4
+  for (int r = threadIdx.x; r < h; r += blockDim.x) {
+    const float a = dy[c * h + r] * (gain ? gain[r] : 1.0f), xh = (x[c * h + r] - m) * rs;
+    dx[c * h + r] = rs * (a - ma - xh * mx);
+  }
+}
+// grid: (blocks of 256 rows, parts of the columns)
+__global__ void __launch_bounds__(256) k_layer_norm_shares(const float* dy, const float* x, const float* stats, float* part, int h, int w) {
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r >= h) return;
+  const long c0 = (long)w * blockIdx.y / gridDim.y, c1 = (long)w * (blockIdx.y + 1) / gridDim.y;
+  float dg = 0.0f, db = 0.0f;
+#pragma unroll 4
+  for (long c = c0; c < c1; c++) {
+    const float d = dy[c * h + r];
+    dg += d * ((x[c * h + r] - stats[2 * c]) * stats[2 * c + 1]);
+    db += d;
+  }
+  part[2L * blockIdx.y * h + r] = dg;
+  part[(2L * blockIdx.y + 1) * h + r] = db;
+}
+
+// The blocks' shares, in order: 32 values a block, eight threads a value.
+__global__ void __launch_bounds__(256) k_layer_norm_params(const float* part, int blocks, float* dgain, float* dbias, int h) {
+  __shared__ float red[8][33];
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const long v = (long)blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (v < 2L * h) {
+#pragma unroll 8
+    for (int b = wid; b < blocks; b += 8) s += part[2L * b * h + v];
+  }
+  red[wid][lane] = s;
+  __syncthreads();
+  if (wid || v >= 2L * h) return;
+#pragma unroll
+  for (int k = 1; k < 8; k++) s += red[k][lane];
+  if (v < h) {
+    if (dgain) dgain[v] = s;
+  } else if (dbias) {
+    dbias[v - h] = s;
+  }
+}
+
+bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+int round32(int n) { return (n + 31) & ~31; }
+
+int vector_ok(const cudamat* v, int h) {
+  if (!v) return 0;
+  if (!v->on_device) return ERROR_NOT_ON_DEVICE;
+  return numel(v) == h && (v->size[0] == 1 || v->size[1] == 1) ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
+}
+
+}  // namespace
+
+extern "C" {
+
+int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, cudamat* stats, float eps) {
+  if (!mat->on_device || !target->on_device || (stats && !stats->on_device)) return ERROR_NOT_ON_DEVICE;
+  if (mat->is_trans || target->is_trans || (stats && stats->is_trans)) return ERROR_TRANSPOSED;
+  const int h = mat->size[0], w = mat->size[1];
+  if (!same_shape(mat, target) || (stats && (stats->size[0] != 2 || stats->size[1] != w))) return ERROR_INCOMPATIBLE_DIMENSIONS;
+  int err = vector_ok(gain, h);
+  if (!err) err = vector_ok(bias, h);
+  if (err) return err;
+  if (!(eps >= 0.0f)) {
+    set_error("eps has to be at least 0");
+    return ERROR_UNSUPPORTED;
+  }
+  if (h == 0 || w == 0) return 0;
+  const float *x = mat->data_device, *g = gain ? gain->data_device : nullptr, *b = bias ? bias->data_device : nullptr;
+  float *y = target->data_device, *st = stats ? stats->data_device : nullptr;
+  const bool vec = h % 4 == 0 && on16(x) && on16(y) && on16(g) && on16(b);
+  const int items = vec ? h / 4 : h;
+#define NORM(VEC, PER, BLOCK, GRID, THREADS) \
+  (void)launch_dependent(k_layer_norm<VEC, PER, BLOCK>, dim3(GRID), dim3(THREADS), 0, stream(), x, g, b, y, st, h, w, eps)
+#define NORM_PER(PER, BLOCK, GRID, THREADS)                \
+  do {                                                     \
+    if (vec) NORM(4, PER, BLOCK, GRID, THREADS);           \
+    else NORM(1, PER, BLOCK, GRID, THREADS);               \
+  } while (0)
+  const int warps = (w + kWarpsPerBlock - 1) / kWarpsPerBlock;
+  if (items <= 32) NORM_PER(1, false, warps, 32 * kWarpsPerBlock);
+  else if (items <= 64) NORM_PER(2, false, warps, 32 * kWarpsPerBlock);
+  else if (items <= 128) NORM_PER(4, false, warps, 32 * kWarpsPerBlock);
+  else if (items <= 256) NORM_PER(8, false, warps, 32 * kWarpsPerBlock);
+  else if (items <= 4 * 1024) NORM_PER(4, true, w, round32((items + 3) / 4));
+  else if (items <= 8 * 1024) NORM_PER(8, true, w, 1024);
+  else (void)launch_dependent(k_layer_norm_long, dim3(w), dim3(1024), 0, stream(), x, g, b, y, st, h, w, eps);
+#undef NORM_PER
+#undef NORM
+  return check_launch();
+}
+
+int layer_norm_deriv(cudamat* deriv, cudamat* mat, cudamat* stats, cudamat* gain, cudamat* target, cudamat* grad_gain,
+                     cudamat* grad_bias) {
+  if (!deriv->on_device || !mat->on_device || !stats->on_device || !target->on_device) return ERROR_NOT_ON_DEVICE;
+  if (deriv->is_trans || mat->is_trans || stats->is_trans || target->is_trans) return ERROR_TRANSPOSED;
+  const int h = mat->size[0], w = mat->size[1];
+  if (!same_shape(mat, deriv) || !same_shape(mat, target) || stats->size[0] != 2 || stats->size[1] != w)
+    return ERROR_INCOMPATIBLE_DIMENSIONS;
+  int err = vector_ok(gain, h);
+  if (!err) err = vector_ok(grad_gain, h);
+  if (!err) err = vector_ok(grad_bias, h);
+  if (err) return err;
+  if (h == 0) return 0;
+  float *dgain = grad_gain ? grad_gain->data_device : nullptr, *dbias = grad_bias ? grad_bias->data_device : nullptr;
+  if (w == 0) {            // sums over no columns
+    for (float* p : {dgain, dbias})
+      if (p && cudaMemsetAsync(p, 0, sizeof(float) * h, stream()) != cudaSuccess) return set_error(cudaGetErrorString(cudaGetLastError()));
+    return 0;
+  }
+  const float *dy = deriv->data_device, *x = mat->data_device, *st = stats->data_device, *g = gain ? gain->data_device : nullptr;
+  float* dx = target->data_device;
+  const bool vec = h % 4 == 0 && on16(dy) && on16(x) && on16(dx) && on16(g), params = dgain || dbias;
+  const int items = vec ? h / 4 : h;
+  // how many blocks the columns are spread over: each adds 8 h bytes of shares, written and read again
+  const bool by_warp = items <= (vec ? 128 : 256);
+  const bool is_long = items > (vec ? 4 * 512 : 16 * 512);
+  const int columns = by_warp ? (w + kWarpsPerBlock - 1) / kWarpsPerBlock : w;
+  int blocks = by_warp ? 4 * sm_count() : 3 * sm_count();
+  if (is_long) blocks = (2 * sm_count() * 256 + h - 1) / h;
+  if (blocks > columns) blocks = columns;
+  if (blocks < 1) blocks = 1;
+  CallScratch room(5, params ? 2 * sizeof(float) * (size_t)h * blocks : 0);
+  float* part = params ? (float*)room.p : nullptr;
+  if (params && !part) return CUDA_ERROR;
+  if (is_long) {
+    if (params)
+      (void)launch_dependent(k_layer_norm_shares, dim3((h + 255) / 256, blocks), dim3(256), 0, stream(), dy, x, st, part, h, w);
+    (void)launch_dependent(k_layer_norm_deriv_long, dim3(w), dim3(1024), 0, stream(), dy, x, st, g, dx, h, w);
+  } else {
+    const size_t smem = by_warp ? 2 * sizeof(float) * h : 0;
+#define DERIV(VEC, PER, BLOCK, THREADS) \
+  (void)launch_dependent(k_layer_norm_deriv<VEC, PER, BLOCK>, dim3(blocks), dim3(THREADS), smem, stream(), dy, x, st, g, dx, part, h, w)
+    if (vec) {
+      if (items <= 32) DERIV(4, 1, false, 32 * kWarpsPerBlock);
+      else if (items <= 64) DERIV(4, 2, false, 32 * kWarpsPerBlock);
+      else if (items <= 128) DERIV(4, 4, false, 32 * kWarpsPerBlock);
+      else if (items <= 2 * 512) DERIV(4, 2, true, round32((items + 1) / 2));
+      else DERIV(4, 4, true, round32((items + 3) / 4));
+    } else {
+      if (items <= 32) DERIV(1, 1, false, 32 * kWarpsPerBlock);
+      else if (items <= 64) DERIV(1, 2, false, 32 * kWarpsPerBlock);
+      else if (items <= 128) DERIV(1, 4, false, 32 * kWarpsPerBlock);
+      else if (items <= 256) DERIV(1, 8, false, 32 * kWarpsPerBlock);
+      else if (items <= 8 * 512) DERIV(1, 8, true, round32((items + 7) / 8));
+      else DERIV(1, 16, true, round32((items + 15) / 16));
+    }
+#undef DERIV
+  }
+  if (params)
+    (void)launch_dependent(k_layer_norm_params, dim3((2 * (unsigned)h + 31) / 32), dim3(256), 0, stream(), part, blocks, dgain, dbias, h);
+  return check_launch();
+}
+
+}  // extern "C"

@@ -1,0 +1,333 @@
+// Log probabilities of given tokens under the softmax of each column of logits, the distribution's entropy and its
+// likeliest tokens, and the gradient.  With m = max z, s = sum exp(z - m), d = z - m:
+//   log p_t = d_t - log s,   H = log s - (sum exp(d) d) / s
+//   dz_i = g (1[i = t] - p_i) - q p_i (log p_i + H)      for gradients g of log p_t and q of H
+// The logits are read once: every thread carries m, s and sum exp(d) d of what it has seen, joined by warps, then by the
+// block.  Bound by HBM (4 bytes a logit forward, 8 back).  The k likeliest are kept sorted across a warp's lanes (k <= 32) by
+// (value, lower index first); a value that beats the warp's k-th is put in its place with two shuffles, which for logits in
+// no order happens k (1 + ln(n / k)) times in n; the warps' lists are joined at the end.
+// A column whose logits are all -inf has no distribution: log p is -inf, H 0 and the gradient 0.  A NaN or +inf among a
+// column's logits makes all its results NaN (its likeliest tokens are then 0, 1, ...).
+#include "common.cuh"
+
+using namespace b200;
+
+namespace {
+
+constexpr int kMostTop = 32;
+
+struct Sums {
+  float m, s, t;          // maximum, sum exp(z - m), sum exp(z - m) (z - m)
+};
+
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+  const float m = fmaxf(a.m, b.m);
+  if (m == -INFINITY) return a.s != a.s ? a : b;             // (nothing but -inf, or NaN)
+  const float da = a.m - m, db = b.m - m;                    // one of them 0
+  const float fa = expf(da), fb = expf(db);
+  Sums r;
+  r.m = m;
+  r.s = a.s * fa + b.s * fb;
+  r.t = fa > 0.0f ? (a.t + da * a.s) * fa : 0.0f * a.s;      // (0 * s: NaN stays)
+  r.t += fb > 0.0f ? (b.t + db * b.s) * fb : 0.0f * b.s;
+  return r;
+}
+
+// The list a warp keeps: lane i holds the i-th likeliest so far.
+struct Top {
+  float v;
+  int i;
+};
+__device__ __forceinline__ bool beats(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+
+// Puts (v, i) of lane `from` where it belongs (it beats the k-th).
+__device__ __forceinline__ void insert(Top& top, float v, int i, int from) {
+  const int lane = threadIdx.x & 31;
+  v = __shfl_sync(0xffffffffu, v, from);
+  i = __shfl_sync(0xffffffffu, i, from);
+  const float pv = __shfl_up_sync(0xffffffffu, top.v, 1);
+  const int pi = __shfl_up_sync(0xffffffffu, top.i, 1);
+  if (beats(v, i, top.v, top.i)) {
+    const bool here = lane == 0 || !beats(v, i, pv, pi);
+    top.v = here ? v : pv;
+    top.i = here ? i : pi;
+  }
+}
+// Offers one value a lane.
+__device__ __forceinline__ void offer(Top& top, int k, float v, int i, float& kv, int& ki) {
+  unsigned who = __ballot_sync(0xffffffffu, beats(v, i, kv, ki));
+  while (who) {
+    const int from = __ffs(who) - 1;
+    insert(top, v, i, from);
+    kv = __shfl_sync(0xffffffffu, top.v, k - 1);
+    ki = __shfl_sync(0xffffffffu, top.i, k - 1);
+    who &= who - 1;
+    who &= __ballot_sync(0xffffffffu, beats(v, i, kv, ki));
+  }
+}
+
+struct LogProbArgs {
+  const float *z, *tokens;
+  float *logp, *entropy, *stats, *top, *top_tokens;
+  int h, w, k;
+};
+
+__device__ __forceinline__ int token_of(float f, int n) {
+  if (!(fabsf(f) < 2147483648.0f)) return -1;
+  int i = (int)f;
+  if (i < 0) i += n;
+  return i < 0 || i >= n ? -1 : i;
+}
+
+// Group i of kVec logits (4: on 16 bytes).
+template <int kVec>
+__device__ __forceinline__ void load(const float* p, long i, float (&v)[kVec]) {
+  if constexpr (kVec == 4) {
+    const float4 x = reinterpret_cast<const float4*>(p)[i];
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  } else {
+    v[0] = p[i];
+  }
+}
+template <int kVec>
+__device__ __forceinline__ void store(float* p, long i, const float (&v)[kVec]) {
+  if constexpr (kVec == 4) reinterpret_cast<float4*>(p)[i] = make_float4(v[0], v[1], v[2], v[3]);
+  else p[i] = v[0];
+}
+
+// kBatch groups of kVec logits of a thread, all read before the first is used.
+template <int kVec, bool kTop>
+__global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a) {
+  constexpr int kBatch = kVec == 4 ? 2 : 8;
+  __shared__ Sums sums[32];
+  __shared__ Top lists[32 * kMostTop];
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const long c = blockIdx.x;
+  const float* col = a.z + c * a.h;
+  Sums s = {-INFINITY, 0.0f, 0.0f};
+  Top top = {-INFINITY, 0x7fffffff};
+  float kv = -INFINITY;
+  int ki = 0x7fffffff;
+  const int items = a.h / kVec;                        // (kVec 4: h is a multiple)
+  for (int base = 0; base < items; base += kBatch * (int)blockDim.x) {
+    float v[kBatch][kVec];
+#pragma unroll
+    for (int b = 0; b < kBatch; b++) {
+      const int i = base + b * (int)blockDim.x + (int)threadIdx.x;
+      if (i < items) {
+        load<kVec>(col, i, v[b]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; j++) v[b][j] = -INFINITY;
+      }
+    }
+    float m = s.m;
+#pragma unroll
+    for (int b = 0; b < kBatch; b++)
+#pragma unroll
+      for (int j = 0; j < kVec; j++) m = fmaxf(m, v[b][j]);
+    if (m > s.m) {
+      const float d = s.m - m, f = expf(d);
+      s.t = f > 0.0f ? (s.t + d * s.s) * f : 0.0f * s.s;
+      s.s *= f;
+      s.m = m;
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; b++)
+#pragma unroll
+      for (int j = 0; j < kVec; j++) {
+        // (a maximum of -inf: nothing to add but a NaN)
+        const float d = v[b][j] == -INFINITY ? -INFINITY : v[b][j] - m, e = expf(d);
+        s.s += e;
+        s.t += e > 0.0f ? e * d : e;
+      }
+    if (kTop) {
+#pragma unroll
+      for (int b = 0; b < kBatch; b++)
+#pragma unroll
+        for (int j = 0; j < kVec; j++) {
+          const int i = base + b * (int)blockDim.x + (int)threadIdx.x;
+          offer(top, a.k, v[b][j], i < items ? kVec * i + j : 0x7fffffff, kv, ki);
+        }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Sums x;
+    x.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+    x.s = __shfl_xor_sync(0xffffffffu, s.s, o);
+    x.t = __shfl_xor_sync(0xffffffffu, s.t, o);
+    s = (threadIdx.x & o) ? join(x, s) : join(s, x);         // (the same order in both lanes: the same bits)
+  }
+  if (lane == 0) sums[wid] = s;
+  if (kTop && lane < a.k) lists[wid * kMostTop + lane] = top;
+  __syncthreads();
+  if (wid) return;
+  s = lane < warps ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Sums x;
+    x.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+    x.s = __shfl_xor_sync(0xffffffffu, s.s, o);
+    x.t = __shfl_xor_sync(0xffffffffu, s.t, o);
+    s = (threadIdx.x & o) ? join(x, s) : join(s, x);
+  }
+  const bool none = s.m == -INFINITY && s.s == s.s, bad = s.s != s.s;
+  const float ls = none ? 0.0f : logf(s.s);
+  const float nan = __int_as_float(0x7fc00000);
+  if (lane == 0) {
+    if (a.logp) {
+      const int t = token_of(a.tokens[c], a.h);
+      a.logp[c] = t < 0 || bad ? nan : none ? -INFINITY : (col[t] - s.m) - ls;
+    }
+    if (a.entropy) a.entropy[c] = bad ? nan : none ? 0.0f : ls - s.t / s.s;
+    if (a.stats) {
+      a.stats[2 * c] = bad ? nan : s.m;
+      a.stats[2 * c + 1] = bad ? nan : ls;
+    }
+  }
+  if (kTop) {
+    for (int x = 1; x < warps; x++) {
+      const Top other = lane < a.k ? lists[x * kMostTop + lane] : Top{-INFINITY, 0x7fffffff};
+      offer(top, a.k, other.v, other.i, kv, ki);
+    }
+    if (lane < a.k) {
+      a.top[c * a.k + lane] = bad ? nan : none ? -INFINITY : (top.v - s.m) - ls;
+      a.top_tokens[c * a.k + lane] = bad ? (float)lane : (float)top.i;
+    }
+  }
+}
+
+// grid.x: columns; grid.y: parts of a column.  A column without weight is not read.
+template <int kVec>
+__global__ void __launch_bounds__(256) k_log_prob_deriv(const float* z, const float* tokens, const float* stats, const float* grad,
+                                                        const float* entropy, const float* grad_entropy, float* dz, int h) {
+  constexpr int kBatch = kVec == 4 ? 2 : 8;
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const long c = blockIdx.x;
+  const float g = grad ? grad[c] : 0.0f, q = grad_entropy ? grad_entropy[c] : 0.0f, H = grad_entropy ? entropy[c] : 0.0f;
+  const float m = stats[2 * c], ls = stats[2 * c + 1];
+  const int t = g != 0.0f ? token_of(tokens[c], h) : -1;
+  const bool zero = (g == 0.0f && q == 0.0f) || m == -INFINITY, bad = g != 0.0f && t < 0;
+  const float* col = z + c * h;
+  float* out = dz + c * h;
+  const int items = h / kVec, step = gridDim.y * blockDim.x;
+  for (int base = blockIdx.y * blockDim.x + threadIdx.x; base < items; base += kBatch * step) {
+    float v[kBatch][kVec];
+#pragma unroll
+    for (int b = 0; b < kBatch; b++) {
+      const int i = base + b * step;
+      if (zero || i >= items) continue;
+      load<kVec>(col, i, v[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; b++) {
+      const int i = base + b * step;
+      if (i >= items) continue;
+#pragma unroll
+      for (int j = 0; j < kVec; j++) {
+        float r = 0.0f;
+        if (!zero) {
+          const float lp = (v[b][j] - m) - ls, p = expf(lp);
+          // -p (g + q (log p + H)), and 0 where p is: log p may be -inf there
+          r = p > 0.0f ? -p * (g + q * (lp + H)) : 0.0f * p;
+          if (kVec * i + j == t) r += g;
+          if (bad) r = __int_as_float(0x7fc00000);
+        }
+        v[b][j] = r;
+      }
+      store<kVec>(out, i, v[b]);
+    }
+  }
+}
+
+// A row of w values.
+int row_ok(const cudamat* v, int w) {
+  if (!v) return 0;
+  if (!v->on_device) return ERROR_NOT_ON_DEVICE;
+  return v->size[0] == 1 && v->size[1] == w ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
+}
+bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int log_prob(cudamat* logits, cudamat* tokens, cudamat* target, cudamat* entropy, cudamat* stats, cudamat* top, cudamat* top_tokens) {
+  if (!logits->on_device || (stats && !stats->on_device) || (top && !top->on_device) || (top_tokens && !top_tokens->on_device))
+    return ERROR_NOT_ON_DEVICE;
+  if (logits->is_trans || (stats && stats->is_trans) || (top && top->is_trans) || (top_tokens && top_tokens->is_trans))
+    return ERROR_TRANSPOSED;
+  const int h = logits->size[0], w = logits->size[1];
+  int err = row_ok(tokens, w);
+  if (!err) err = row_ok(target, w);
+  if (!err) err = row_ok(entropy, w);
+  if (err) return err;
+  if ((stats && (stats->size[0] != 2 || stats->size[1] != w)) || !top != !top_tokens ||
+      (top && (!same_shape(top, top_tokens) || top->size[1] != w || top->size[0] > h)) || !tokens != !target)
+    return ERROR_INCOMPATIBLE_DIMENSIONS;
+  if (w == 0) return 0;
+  if (h == 0 || h > (1 << 24) || (top && top->size[0] > kMostTop)) {
+    set_error(h == 0 ? "columns without a logit have no distribution"
+                     : h > (1 << 24) ? "a float32 does not hold every token of a column" : "at most 32 top tokens a column");
+    return ERROR_UNSUPPORTED;
+  }
+  LogProbArgs a;
+  auto at = [](cudamat* v) { return v ? v->data_device : nullptr; };
+  a.z = logits->data_device;
+  a.tokens = at(tokens);
+  a.logp = at(target);
+  a.entropy = at(entropy);
+  a.stats = at(stats);
+  a.top = at(top);
+  a.top_tokens = at(top_tokens);
+  a.h = h;
+  a.w = w;
+  a.k = top ? top->size[0] : 0;
+  const bool vec = h % 4 == 0 && on16(a.z);
+  // as many warps a column as fill the device, with eight logits a thread or more
+  int warps = 1;
+  while (warps < 32 && (long)w * warps < 32L * sm_count() && (long)warps * 32 * 8 < h) warps *= 2;
+#define LOGP(VEC, TOP) (void)launch_dependent(k_log_prob<VEC, TOP>, dim3(w), dim3(32 * warps), 0, stream(), a)
+  if (vec && a.k) LOGP(4, true);
+  else if (vec) LOGP(4, false);
+  else if (a.k) LOGP(1, true);
+  else LOGP(1, false);
+#undef LOGP
+  return check_launch();
+}
+
+int log_prob_deriv(cudamat* logits, cudamat* tokens, cudamat* stats, cudamat* grad, cudamat* entropy, cudamat* grad_entropy,
+                   cudamat* target) {
+  if (!logits->on_device || !stats->on_device || !target->on_device) return ERROR_NOT_ON_DEVICE;
+  if (logits->is_trans || stats->is_trans || target->is_trans) return ERROR_TRANSPOSED;
+  const int h = logits->size[0], w = logits->size[1];
+  int err = row_ok(tokens, w);
+  if (!err) err = row_ok(grad, w);
+  if (!err) err = row_ok(entropy, w);
+  if (!err) err = row_ok(grad_entropy, w);
+  if (err) return err;
+  if (!same_shape(logits, target) || stats->size[0] != 2 || stats->size[1] != w || (grad && !tokens) || (grad_entropy && !entropy))
+    return ERROR_INCOMPATIBLE_DIMENSIONS;
+  if (h == 0 || w == 0) return 0;
+  auto at = [](cudamat* v) { return v ? v->data_device : nullptr; };
+  const float* z = logits->data_device;
+  float* dz = target->data_device;
+  const bool vec = h % 4 == 0 && on16(z) && on16(dz);
+  const int per_block = 256 * 8;                         // logits of a block's batch
+  int parts = (h + per_block - 1) / per_block;
+  while (parts > 1 && (long)w * parts > 16L * sm_count()) parts = (parts + 1) / 2;
+  const dim3 grid(w, parts);
+  if (vec)
+    (void)launch_dependent(k_log_prob_deriv<4>, grid, dim3(256), 0, stream(), z, at(tokens), stats->data_device, at(grad), at(entropy),
+                           at(grad_entropy), dz, h);
+  else
+    (void)launch_dependent(k_log_prob_deriv<1>, grid, dim3(256), 0, stream(), z, at(tokens), stats->data_device, at(grad), at(entropy),
+                           at(grad_entropy), dz, h);
+  return check_launch();
+}
+
+}  // extern "C"

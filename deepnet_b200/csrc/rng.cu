@@ -73,7 +73,102 @@ int launch(rnd_struct* rnd, cudamat* mat, cudamat* target, float p0 = 0, float p
   return check_launch();
 }
 
+// target = add + (u > p ? mat * scale : 0).  The comparison is made on the random word itself: its uniform grows with it, so
+// `last`, the largest word that is dropped, decides as u > p does.  A thread takes kRows rows of four columns.
+// Bound by HBM (8 bytes an element, 12 with `add`) with the Philox rounds close behind: they and the mask take about 25
+// instructions an element of the 40 or so that fit beside 8 bytes.
+template <int kRows, bool kAdd>
+__global__ void __launch_bounds__(256) k_dropout_scaled(const float* src, const float* add, float* dst, int h, int w, int col0,
+                                                        PhiloxKey key, uint32_t last, bool all, float scale) {
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int groups = h / kRows, blk0 = col0 >> 2;
+  const long it = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  const int b = (int)(it / groups), r = kRows * (int)(it - (long)b * groups);
+  const int c0 = ((blk0 + b) << 2) - col0;         // first local column (below 0, or the last beyond w, at a shard's ends)
+  if (c0 >= w) return;
+  float x[4][kRows], y[4][kRows];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int c = c0 + j;
+    if (c < 0 || c >= w) continue;
+    const long idx = (long)c * h + r;
+    if constexpr (kRows == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(src + idx);
+      x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+      if (kAdd) {
+        const float4 a = *reinterpret_cast<const float4*>(add + idx);
+        y[j][0] = a.x; y[j][1] = a.y; y[j][2] = a.z; y[j][3] = a.w;
+      }
+    } else {
+      x[j][0] = src[idx];
+      if (kAdd) y[j][0] = add[idx];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; i++) {
+    const uint4 wd = philox4x32_10((uint32_t)(r + i), (uint32_t)(blk0 + b), key);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float kept = pick_word(wd, j) > last || all ? x[j][i] * scale : 0.0f;
+      y[j][i] = kAdd ? y[j][i] + kept : kept;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int c = c0 + j;
+    if (c < 0 || c >= w) continue;
+    const long idx = (long)c * h + r;
+    if constexpr (kRows == 4) *reinterpret_cast<float4*>(dst + idx) = make_float4(y[j][0], y[j][1], y[j][2], y[j][3]);
+    else dst[idx] = y[j][0];
+  }
+}
+
+// The uniform of a word as the device computes it.
+float uniform_of(uint32_t word) {
+  const volatile float f = (float)word;
+  const volatile float g = f + 1.0f;
+  return g * 2.3283064365386963e-10f;
+}
+
 }  // namespace
+
+extern "C" {
+
+int dropout_scaled(rnd_struct* rnd_state, cudamat* mat, cudamat* add, cudamat* target, float dropprob) {
+  if (!mat->on_device || !target->on_device || (add && !add->on_device)) return ERROR_NOT_ON_DEVICE;
+  if (mat->is_trans || target->is_trans || (add && add->is_trans)) return ERROR_TRANSPOSED;
+  if (!same_shape(mat, target) || (add && !same_shape(mat, add))) return ERROR_INCOMPATIBLE_DIMENSIONS;
+  if (!(dropprob >= 0.0f && dropprob <= 1.0f)) {
+    set_error("the probability has to lie in 0 .. 1");
+    return ERROR_UNSUPPORTED;
+  }
+  const PhiloxKey key = make_philox_key(rnd_state->seed, rnd_state->calls);
+  rnd_state->calls += 1;
+  const int h = mat->size[0], w = mat->size[1], col0 = rng_col0();
+  if ((long)h * w == 0) return 0;
+  // largest word whose uniform is not above dropprob (word 0 is above 0 already: then everything is kept)
+  uint32_t last = 0;
+  const bool all = uniform_of(0) > dropprob;
+  for (uint32_t bit = 1u << 31; bit && !all; bit >>= 1)
+    if (!(uniform_of(last | bit) > dropprob)) last |= bit;
+  const float scale = dropprob < 1.0f ? (float)(1.0 / (1.0 - (double)dropprob)) : 0.0f;
+  const float *x = mat->data_device, *a = add ? add->data_device : nullptr;
+  float* y = target->data_device;
+  const bool vec = h % 4 == 0 && (((uintptr_t)x | (uintptr_t)a | (uintptr_t)y) & 15) == 0;
+  const long items = (long)(vec ? h / 4 : h) * (((col0 + (long)w - 1) >> 2) - (col0 >> 2) + 1);
+  const dim3 grid((unsigned)((items + 255) / 256));
+#define DROP(ROWS, ADD) \
+  (void)launch_dependent(k_dropout_scaled<ROWS, ADD>, grid, dim3(256), 0, stream(), x, a, y, h, w, col0, key, last, all, scale)
+  if (vec && a) DROP(4, true);
+  else if (vec) DROP(4, false);
+  else if (a) DROP(1, true);
+  else DROP(1, false);
+#undef DROP
+  return check_launch();
+}
+
+}  // extern "C"
 
 extern "C" {
 

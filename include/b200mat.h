@@ -292,6 +292,30 @@ int sample_multinomial(rnd_struct* rnd_state, cudamat* probs, cudamat* nn, cudam
  * deepnet/logistic_layer.py:48-52 without the host round trip). */
 int add_sq_diff(cudamat* a, cudamat* b, cudamat* acc);
 
+/* ---- layers trained by gradients, words scored (no counterpart in the reference) ------ */
+/* Columns normalised: target = gain (x - mean) / sqrt(variance + eps) + bias, column by column; gain and bias (one value a row)
+ * may be null, target may be mat.  stats (2 x columns, or null) receives mean and 1 / sqrt(variance + eps) for the derivative. */
+int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, cudamat* stats, float eps);
+/* deriv: the gradient of layer_norm's target; mat, stats, gain: what it was given and gave.  target (may be deriv or mat) = the
+ * gradient of mat; grad_gain, grad_bias (one value a row, or null) = those of gain and bias, summed over columns in a fixed order. */
+int layer_norm_deriv(cudamat* deriv, cudamat* mat, cudamat* stats, cudamat* gain, cudamat* target, cudamat* grad_gain, cudamat* grad_bias);
+
+/* target = add + (u > dropprob ? mat / (1 - dropprob) : 0), add (or null: 0) of mat's shape, u the uniforms that fill_with_rand would
+ * draw.  Consumes one sampling call.  No mask is stored: the same seed and call number draw it again (on the gradient: without add).
+ * target may be mat or add.  dropprob 1 drops everything, 0 nothing. */
+int dropout_scaled(rnd_struct* rnd_state, cudamat* mat, cudamat* add, cudamat* target, float dropprob);
+
+/* Of the softmax of every column of logits (V x N): target (1 x N) = log probability of its token (tokens: 1 x N float32 holding
+ * integers, negative ones count from the end; one out of range gives NaN); entropy (1 x N); stats (2 x N: maximum, log of the sum of
+ * exponentials above it, for the derivative); top, top_tokens (k x N, k <= 32 and <= V): log probabilities and numbers of the k
+ * likeliest, likeliest first, of equal logits the lower number.  Each output may be null (target and tokens, top and top_tokens
+ * together).  A column of -inf alone: -inf, entropy 0; a NaN or +inf in it: NaN, and tokens 0, 1, ... .  V <= 2^24. */
+int log_prob(cudamat* logits, cudamat* tokens, cudamat* target, cudamat* entropy, cudamat* stats, cudamat* top, cudamat* top_tokens);
+/* target (may be logits) = gradient of the logits, from grad (1 x N, or null), the gradient of log_prob's target, and grad_entropy
+ * (1 x N, or null; with entropy as log_prob gave it), that of its entropy.  A column whose gradients are 0 gives 0 whatever its
+ * logits and token are, and so does one of -inf alone. */
+int log_prob_deriv(cudamat* logits, cudamat* tokens, cudamat* stats, cudamat* grad, cudamat* entropy, cudamat* grad_entropy, cudamat* target);
+
 /* Library control. */
 int b200_device_count(void);
 int b200_set_stream(void* cuda_stream);   /* NULL restores the library's own stream; scratch is kept per stream, for that

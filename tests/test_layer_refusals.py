@@ -1,0 +1,97 @@
+"""What layer normalisation, dropout by key and log probabilities refuse.  The checks come before anything touches a device, so
+they are tested without one, on handles that name no memory."""
+import ctypes as ct
+
+import pytest
+
+from deepnet_b200 import b200mat as cm
+
+DIMENSIONS, TRANSPOSED, NOT_ON_DEVICE, UNSUPPORTED = -1, -5, -8, -9
+
+
+def mat(rows, cols, on_device=1, trans=0):
+    m = cm.cudamat()
+    m.size[0], m.size[1], m.on_device, m.is_trans = rows, cols, on_device, trans
+    m.data_device = ct.cast(0, ct.POINTER(ct.c_float))
+    return ct.pointer(m)
+
+
+def norm(x, gain, bias, y, stats, eps=1e-5):
+    return cm._lib.layer_norm(x, gain, bias, y, stats, ct.c_float(eps))
+
+
+def test_layer_norm_refuses():
+    x = lambda **k: mat(8, 5, **k)
+    assert norm(x(), None, None, mat(8, 4), None) == DIMENSIONS
+    assert norm(x(), mat(7, 1), None, x(), None) == DIMENSIONS
+    assert norm(x(), mat(4, 2), None, x(), None) == DIMENSIONS          # eight values, but no vector
+    assert norm(x(), None, mat(1, 9), x(), None) == DIMENSIONS
+    assert norm(x(), None, None, x(), mat(5, 2)) == DIMENSIONS
+    assert norm(x(trans=1), None, None, x(), None) == TRANSPOSED
+    assert norm(x(), None, None, x(trans=1), None) == TRANSPOSED
+    assert norm(x(on_device=0), None, None, x(), None) == NOT_ON_DEVICE
+    assert norm(x(), mat(8, 1, on_device=0), None, x(), None) == NOT_ON_DEVICE
+    for eps in (-1e-5, float("nan")):
+        assert norm(x(), None, None, x(), None, eps) == UNSUPPORTED
+    assert norm(mat(0, 5), None, None, mat(0, 5), None) == 0 and norm(mat(8, 0), None, None, mat(8, 0), mat(2, 0)) == 0
+
+
+def test_layer_norm_deriv_refuses():
+    f = cm._lib.layer_norm_deriv
+    x, st = (lambda **k: mat(8, 5, **k)), (lambda **k: mat(2, 5, **k))
+    assert f(mat(8, 4), x(), st(), None, x(), None, None) == DIMENSIONS
+    assert f(x(), x(), mat(1, 5), None, x(), None, None) == DIMENSIONS
+    assert f(x(), x(), st(), None, mat(5, 8), None, None) == DIMENSIONS
+    assert f(x(), x(), st(), mat(5, 1), x(), None, None) == DIMENSIONS
+    assert f(x(), x(), st(), None, x(), mat(9, 1), None) == DIMENSIONS
+    assert f(x(), x(), st(), None, x(), None, mat(1, 7)) == DIMENSIONS
+    assert f(x(trans=1), x(), st(), None, x(), None, None) == TRANSPOSED
+    assert f(x(), x(), st(on_device=0), None, x(), None, None) == NOT_ON_DEVICE
+
+
+def test_dropout_scaled_refuses_and_draws_nothing():
+    def f(x, add, y, p=0.5):
+        state = cm.rnd_struct(3, 7)
+        err = cm._lib.dropout_scaled(ct.byref(state), x, add, y, ct.c_float(p))
+        assert (state.seed, state.calls) == (3, 8 if err == 0 else 7)
+        return err
+    assert f(mat(4, 3), None, mat(3, 4)) == DIMENSIONS
+    assert f(mat(4, 3), mat(4, 2), mat(4, 3)) == DIMENSIONS
+    assert f(mat(4, 3, trans=1), None, mat(4, 3)) == TRANSPOSED
+    assert f(mat(4, 3), mat(4, 3, trans=1), mat(4, 3)) == TRANSPOSED
+    assert f(mat(4, 3), None, mat(4, 3, on_device=0)) == NOT_ON_DEVICE
+    for p in (-0.1, 1.5, float("nan")):
+        assert f(mat(4, 3), None, mat(4, 3), p) == UNSUPPORTED
+    assert f(mat(0, 3), None, mat(0, 3)) == 0
+
+
+def test_log_prob_refuses():
+    f = cm._lib.log_prob
+    z, row = (lambda **k: mat(10, 6, **k)), (lambda **k: mat(1, 6, **k))
+    assert f(z(), mat(1, 5), row(), None, None, None, None) == DIMENSIONS
+    assert f(z(), mat(6, 1), row(), None, None, None, None) == DIMENSIONS
+    assert f(z(), row(), None, None, None, None, None) == DIMENSIONS               # a token without a place for its result
+    assert f(z(), None, row(), None, None, None, None) == DIMENSIONS
+    assert f(z(), row(), row(), mat(1, 7), None, None, None) == DIMENSIONS
+    assert f(z(), row(), row(), None, mat(6, 2), None, None) == DIMENSIONS
+    assert f(z(), row(), row(), None, None, mat(3, 6), None) == DIMENSIONS
+    assert f(z(), row(), row(), None, None, mat(3, 6), mat(2, 6)) == DIMENSIONS
+    assert f(z(), row(), row(), None, None, mat(11, 6), mat(11, 6)) == DIMENSIONS  # more of them than tokens
+    assert f(mat(40, 6), None, None, None, None, mat(33, 6), mat(33, 6)) == UNSUPPORTED
+    assert f(mat(0, 6), row(), row(), None, None, None, None) == UNSUPPORTED
+    assert f(mat((1 << 24) + 1, 6), row(), row(), None, None, None, None) == UNSUPPORTED
+    assert f(z(trans=1), row(), row(), None, None, None, None) == TRANSPOSED
+    assert f(z(on_device=0), row(), row(), None, None, None, None) == NOT_ON_DEVICE
+    assert f(z(), row(on_device=0), row(), None, None, None, None) == NOT_ON_DEVICE
+    assert f(mat(10, 0), mat(1, 0), mat(1, 0), None, None, None, None) == 0
+
+
+def test_log_prob_deriv_refuses():
+    f = cm._lib.log_prob_deriv
+    z, row, st = (lambda **k: mat(10, 6, **k)), (lambda: mat(1, 6)), (lambda: mat(2, 6))
+    assert f(z(), row(), st(), row(), None, None, mat(10, 5)) == DIMENSIONS
+    assert f(z(), row(), mat(2, 5), row(), None, None, z()) == DIMENSIONS
+    assert f(z(), None, st(), row(), None, None, z()) == DIMENSIONS                # a gradient of log probabilities of no tokens
+    assert f(z(), row(), st(), row(), None, row(), z()) == DIMENSIONS              # a gradient of entropies that are not given
+    assert f(z(trans=1), row(), st(), row(), None, None, z()) == TRANSPOSED
+    assert f(z(), row(), st(), row(), None, None, z(on_device=0)) == NOT_ON_DEVICE
