@@ -893,6 +893,34 @@ def fused_gemm(passes, out=None, sample=None, bias=None, col_scale=None, activat
         sample_aux.form = None
 
 
+GATED_ACTIVATIONS = ("linear", "logistic", "relu", "silu", "gelu")
+
+
+def _gated_activation(name):
+    if name not in GATED_ACTIVATIONS:
+        raise CUDAMatException("activation has to be one of %s" % ", ".join(GATED_ACTIVATIONS))
+    return ct.c_int(GATED_ACTIVATIONS.index(name))
+
+
+def gated_product(gate_w, up_w, mat, target=None, activation="logistic", gate_bias=None, up_bias=None, gate=None, up=None):
+    """target = act(gate_w' mat + gate_bias) * (up_w' mat + up_bias) in one kernel: a gated layer's forward pass.  Weights are inputs x
+    units, mat inputs x cases; activation one of `GATED_ACTIVATIONS` (silu: g logistic(g), gelu: g Phi(g)).  gate and up (units x
+    cases, both or neither) receive the two sums, which `gated_product_deriv` needs."""
+    if target is None:
+        target = empty((gate_w.shape[1], mat.shape[1]))
+    _check(_lib.gated_product(gate_w.p_mat, up_w.p_mat, mat.p_mat, _p(gate_bias), _p(up_bias), _gated_activation(activation), _p(gate),
+                              _p(up), target.p_mat))
+    return target
+
+
+def gated_product_deriv(deriv, gate, up, gate_w, up_w, mat, activation="logistic", grad_x=None, grad_gate_w=None, grad_up_w=None,
+                        grad_gate_bias=None, grad_up_bias=None):
+    """deriv is the gradient of `gated_product`'s target.  gate and up, as that call left them, are overwritten with their gradients;
+    the gradients of mat, weights and biases go to the matrices given for them."""
+    _check(_lib.gated_product_deriv(deriv.p_mat, gate.p_mat, up.p_mat, gate_w.p_mat, up_w.p_mat, mat.p_mat, _gated_activation(activation),
+                                    _p(grad_x), _p(grad_gate_w), _p(grad_up_w), _p(grad_gate_bias), _p(grad_up_bias)))
+
+
 def _build_bias_layers(layers, sq_acc):
     t = _BiasLayers()
     t.layers = len(layers)

@@ -300,6 +300,16 @@ int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, cuda
  * gradient of mat; grad_gain, grad_bias (one value a row, or null) = those of gain and bias, summed over columns in a fixed order. */
 int layer_norm_deriv(cudamat* deriv, cudamat* mat, cudamat* stats, cudamat* gain, cudamat* target, cudamat* grad_gain, cudamat* grad_bias);
 
+/* A gated layer: target (H x N) = act(gate_w' mat + gate_bias) * (up_w' mat + up_bias), weights V x H, mat V x N, biases (one value a
+ * unit) or null; activation 0 none, 1 logistic, 2 max(0, g), 3 g logistic(g), 4 g Phi(g).  gate and up (H x N, both or neither) receive
+ * the sums the activation is taken of, for the derivative. */
+int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bias, cudamat* up_bias, int activation, cudamat* gate,
+                  cudamat* up, cudamat* target);
+/* deriv: the gradient of gated_product's target.  gate and up, as it left them, are overwritten with their gradients; the others
+ * receive those of mat, weights and biases (null: not wanted), summed in a fixed order. */
+int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gate_w, cudamat* up_w, cudamat* mat, int activation,
+                        cudamat* grad_mat, cudamat* grad_gate_w, cudamat* grad_up_w, cudamat* grad_gate_bias, cudamat* grad_up_bias);
+
 /* target = add + (u > dropprob ? mat / (1 - dropprob) : 0), add (or null: 0) of mat's shape, u the uniforms that fill_with_rand would
  * draw.  Consumes one sampling call.  No mask is stored: the same seed and call number draw it again (on the gradient: without add).
  * target may be mat or add.  dropprob 1 drops everything, 0 nothing. */

@@ -95,3 +95,35 @@ def test_log_prob_deriv_refuses():
     assert f(z(), row(), st(), row(), None, row(), z()) == DIMENSIONS              # a gradient of entropies that are not given
     assert f(z(trans=1), row(), st(), row(), None, None, z()) == TRANSPOSED
     assert f(z(), row(), st(), row(), None, None, z(on_device=0)) == NOT_ON_DEVICE
+
+
+def test_gated_product_refuses():
+    def f(wg, wu, x, bg=None, bu=None, act=1, gate=None, up=None, y=None):
+        return cm._lib.gated_product(wg, wu, x, bg, bu, ct.c_int(act), gate, up, y if y is not None else mat(7, 5))
+    w, x = (lambda **k: mat(9, 7, **k)), (lambda **k: mat(9, 5, **k))
+    assert f(w(), mat(9, 6), x()) == DIMENSIONS
+    assert f(w(), w(), mat(8, 5)) == DIMENSIONS
+    assert f(w(), w(), x(), y=mat(7, 4)) == DIMENSIONS
+    assert f(w(), w(), x(), bg=mat(9, 1)) == DIMENSIONS
+    assert f(w(), w(), x(), bu=mat(7, 2)) == DIMENSIONS
+    assert f(w(), w(), x(), gate=mat(7, 5)) == DIMENSIONS               # one of the two sums
+    assert f(w(), w(), x(), gate=mat(7, 5), up=mat(5, 7)) == DIMENSIONS
+    assert f(w(trans=1), w(), x()) == TRANSPOSED and f(w(), w(), x(trans=1)) == TRANSPOSED
+    assert f(w(), w(on_device=0), x()) == NOT_ON_DEVICE and f(w(), w(), x(), y=mat(7, 5, on_device=0)) == NOT_ON_DEVICE
+    assert f(w(), w(), x(), act=-1) == UNSUPPORTED and f(w(), w(), x(), act=5) == UNSUPPORTED
+    assert f(w(), w(), mat(9, 0), y=mat(7, 0)) == 0
+    with pytest.raises(cm.CUDAMatException):
+        cm._gated_activation("softmax")
+
+
+def test_gated_product_deriv_refuses():
+    def f(dy=None, gate=None, up=None, wg=None, wu=None, x=None, act=1, out=(None,) * 5):
+        d = lambda m, r, c: m if m is not None else mat(r, c)
+        return cm._lib.gated_product_deriv(d(dy, 7, 5), d(gate, 7, 5), d(up, 7, 5), d(wg, 9, 7), d(wu, 9, 7), d(x, 9, 5), ct.c_int(act), *out)
+    assert f(dy=mat(7, 4)) == DIMENSIONS and f(up=mat(5, 7)) == DIMENSIONS and f(wu=mat(7, 9)) == DIMENSIONS
+    assert f(out=(mat(9, 4), None, None, None, None)) == DIMENSIONS
+    assert f(out=(None, mat(7, 9), None, None, None)) == DIMENSIONS
+    assert f(out=(None, None, None, mat(9, 1), None)) == DIMENSIONS
+    assert f(gate=mat(7, 5, trans=1)) == TRANSPOSED and f(out=(None, None, mat(9, 7, trans=1), None, None)) == TRANSPOSED
+    assert f(x=mat(9, 5, on_device=0)) == NOT_ON_DEVICE and f(out=(None, None, None, None, mat(7, 1, on_device=0))) == NOT_ON_DEVICE
+    assert f(act=9) == UNSUPPORTED
