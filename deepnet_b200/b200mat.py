@@ -902,14 +902,32 @@ def _gated_activation(name):
     return ct.c_int(GATED_ACTIVATIONS.index(name))
 
 
-def gated_product(gate_w, up_w, mat, target=None, activation="logistic", gate_bias=None, up_bias=None, gate=None, up=None):
+class GatedPlanes(object):
+    """A gated layer's weights in the form its tensor-core products read (`gated_planes` in b200mat.h), for layers that run many times
+    between changes of their weights: as of this call, or of the last `fill`."""
+
+    def __init__(self, gate_w, up_w):
+        if gate_w.shape != up_w.shape:
+            raise CUDAMatException("Incompatible matrix dimensions.")
+        self.gate, self.up, self.scales = AuxMatrix(gate_w.shape), AuxMatrix(up_w.shape), empty((2, gate_w.shape[1]))
+        self.fill(gate_w, up_w)
+
+    def fill(self, gate_w, up_w):
+        """After the weights have changed."""
+        _check(_lib.gated_planes(gate_w.p_mat, up_w.p_mat, self.gate.p_mat, self.up.p_mat, self.scales.p_mat))
+        return self
+
+
+def gated_product(gate_w, up_w, mat, target=None, activation="logistic", gate_bias=None, up_bias=None, gate=None, up=None, planes=None):
     """target = act(gate_w' mat + gate_bias) * (up_w' mat + up_bias) in one kernel: a gated layer's forward pass.  Weights are inputs x
     units, mat inputs x cases; activation one of `GATED_ACTIVATIONS` (silu: g logistic(g), gelu: g Phi(g)).  gate and up (units x
-    cases, both or neither) receive the two sums, which `gated_product_deriv` needs."""
+    cases, both or neither) receive the two sums, which `gated_product_deriv` needs.  planes: the weights' `GatedPlanes`; without
+    them a product that runs on the tensor cores splits the weights every time."""
     if target is None:
         target = empty((gate_w.shape[1], mat.shape[1]))
-    _check(_lib.gated_product(gate_w.p_mat, up_w.p_mat, mat.p_mat, _p(gate_bias), _p(up_bias), _gated_activation(activation), _p(gate),
-                              _p(up), target.p_mat))
+    _check(_lib.gated_product(gate_w.p_mat, up_w.p_mat, mat.p_mat, _p(gate_bias), _p(up_bias), _gated_activation(activation),
+                              *((m.p_mat for m in (planes.gate, planes.up, planes.scales)) if planes is not None else (None,) * 3),
+                              _p(gate), _p(up), target.p_mat))
     return target
 
 

@@ -2,7 +2,8 @@
 // and the derivative.  Weights are inputs x units, as an edge's; x is inputs x cases.
 //   G = Wg' x + bg,  U = Wu' x + bu,  y = act(G) U
 //   dU = dy act(G),  dG = dy U act'(G),  dx = Wg dG + Wu dU,  dWg = x dG',  dWu = x dU',  dbg, dbu: row sums of dG, dU
-#include "common.cuh"
+#include "gated.cuh"
+#include "gemm.cuh"
 
 using namespace b200;
 
@@ -12,29 +13,6 @@ int sum_by_axis(cudamat* mat, cudamat* target, int axis);
 }
 
 namespace {
-
-enum { kLinear = 0, kLogistic, kRelu, kSilu, kGelu, kActivations };
-
-// act(g) and its slope.
-template <int kAct>
-__device__ __forceinline__ float activate(float g, float& slope) {
-  if (kAct == kLogistic || kAct == kSilu) {
-    const float p = sigmoid_accurate(g), q = sigmoid_accurate(-g);     // (1 - p loses what is left of it)
-    slope = kAct == kLogistic ? p * q : p * (1.0f + g * q);
-    return kAct == kLogistic ? p : g * p;
-  }
-  if (kAct == kRelu) {
-    slope = g > 0.0f ? 1.0f : g == g ? 0.0f : g;                       // (NaN stays)
-    return g > 0.0f || g != g ? g : 0.0f;
-  }
-  if (kAct == kGelu) {
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-    slope = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
-    return g * cdf;
-  }
-  slope = 1.0f;
-  return g;
-}
 
 struct GatedArgs {
   const float *wg, *wu, *x, *bg, *bu;
@@ -123,21 +101,46 @@ int bias_ok(const cudamat* v, int h) {
   return numel(v) == h && (v->size[0] == 1 || v->size[1] == 1) ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
 }
 bool is(const cudamat* m, int rows, int cols) { return m->size[0] == rows && m->size[1] == cols; }
-bool is_planes(const cudamat* m, int rows, int cols) { return m->on_device && !m->is_trans && is(m, aux_rows(rows), cols); }
+constexpr long kTensorWork = 1L << 21;      // multiply-adds of one of the products from which the tensor cores take both
 int weights_ok(const cudamat* gate_w, const cudamat* up_w) {
   if (!gate_w->on_device || !up_w->on_device) return ERROR_NOT_ON_DEVICE;
   if (gate_w->is_trans || up_w->is_trans) return ERROR_TRANSPOSED;
   return same_shape(gate_w, up_w) ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
+}
+// Planes of both weights: all three, on 16 bytes.
+int planes_ok(const cudamat* w, const cudamat* gate_planes, const cudamat* up_planes, const cudamat* scales) {
+  if (!gate_planes || !up_planes || !scales) return ERROR_INCOMPATIBLE_DIMENSIONS;
+  if (!gate_planes->on_device || !up_planes->on_device || !scales->on_device) return ERROR_NOT_ON_DEVICE;
+  if (gate_planes->is_trans || up_planes->is_trans || scales->is_trans) return ERROR_TRANSPOSED;
+  const int lda = aux_rows(w->size[0]), H = w->size[1];
+  if (!is(gate_planes, lda, H) || !is(up_planes, lda, H) || !is(scales, 2, H)) return ERROR_INCOMPATIBLE_DIMENSIONS;
+  if (!on16(gate_planes->data_device) || !on16(up_planes->data_device)) {
+    set_error("planes have to start on 16 bytes");
+    return ERROR_UNSUPPORTED;
+  }
+  return 0;
 }
 
 }  // namespace
 
 extern "C" {
 
-int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bias, cudamat* up_bias, int activation, cudamat* gate,
-                  cudamat* up, cudamat* target) {
+int gated_planes(cudamat* gate_w, cudamat* up_w, cudamat* gate_planes, cudamat* up_planes, cudamat* scales) {
+  int err = weights_ok(gate_w, up_w);
+  if (!err) err = planes_ok(gate_w, gate_planes, up_planes, scales);
+  if (err) return err;
+  const int V = gate_w->size[0], H = gate_w->size[1];
+  if (V == 0 || H == 0) return 0;
+  const SplitJob jobs[2] = {{gate_w->data_device, (uint16_t*)gate_planes->data_device, scales->data_device, 2, H},
+                            {up_w->data_device, (uint16_t*)up_planes->data_device, scales->data_device + 1, 2, H}};
+  return split_columns(jobs, 2, V);
+}
+
+int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bias, cudamat* up_bias, int activation,
+                  cudamat* gate_planes, cudamat* up_planes, cudamat* scales, cudamat* gate, cudamat* up, cudamat* target) {
   int err = weights_ok(gate_w, up_w);
   if (err) return err;
+  if ((gate_planes || up_planes || scales) && (err = planes_ok(gate_w, gate_planes, up_planes, scales))) return err;
   if (!mat->on_device || !target->on_device || (gate && !gate->on_device) || (up && !up->on_device)) return ERROR_NOT_ON_DEVICE;
   if (mat->is_trans || target->is_trans || (gate && gate->is_trans) || (up && up->is_trans)) return ERROR_TRANSPOSED;
   const int V = gate_w->size[0], H = gate_w->size[1], N = mat->size[1];
@@ -150,6 +153,34 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
   }
   if (H == 0 || N == 0) return 0;
   auto at = [](cudamat* m) { return m ? m->data_device : nullptr; };
+  // Tensor cores, behind a launch or two that split the operands: where the products are more than those cost.
+  const bool large = (long)V * H * N >= kTensorWork;
+  if (V > 0 && gemm_path() != 2 && (large || gemm_path() == 1) && tma_available()) {
+    const long px = (long)aux_rows(V) * N * 4, pw = gate_planes ? 0 : (long)aux_rows(V) * H * 4;
+    const long inv = ((long)(N + 2L * H) * 4 + 255) / 256 * 256;
+    CallScratch room(6, (size_t)(px + 2 * pw + inv));
+    if (!room.p) return CUDA_ERROR;
+    uint16_t* xp = (uint16_t*)((char*)room.p + inv);
+    float* x_inv = (float*)room.p;
+    GatedForward f;
+    f.x = {xp, V, N};
+    f.wg = {gate_planes ? (uint16_t*)gate_planes->data_device : xp + px / 2, V, H};
+    f.wu = {gate_planes ? (uint16_t*)up_planes->data_device : xp + (px + pw) / 2, V, H};
+    float* w_inv = gate_planes ? scales->data_device : x_inv + N;
+    const SplitJob jobs[3] = {{mat->data_device, xp, x_inv, 1, N},
+                              {gate_w->data_device, (uint16_t*)f.wg.p, w_inv, 2, H},
+                              {up_w->data_device, (uint16_t*)f.wu.p, w_inv + 1, 2, H}};
+    if ((err = split_columns(jobs, gate_planes ? 1 : 3, V))) return err;
+    f.w_inv = w_inv;
+    f.x_inv = x_inv;
+    f.bg = at(gate_bias);
+    f.bu = at(up_bias);
+    f.gate = at(gate);
+    f.up = at(up);
+    f.y = target->data_device;
+    f.activation = activation;
+    return gated_tc(f);
+  }
   const GatedArgs a = {gate_w->data_device, up_w->data_device, mat->data_device, at(gate_bias), at(up_bias),
                        at(gate),            at(up),            target->data_device, V, H, N};
   const long tiles = (long)((H + 63) / 64) * ((N + 63) / 64);

@@ -3,6 +3,8 @@
 // with an optional Bernoulli draw of the result, and optionally the aux matrices (bfloat16
 // parts) of result and draw for the products that read them next.
 #pragma once
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace b200 {
@@ -91,6 +93,11 @@ int rewrite_f16_planes_if(const float* x, uint16_t* aux, int rows, long n, const
 // the peers' receive buffers here, so that its statistics reach their owners while the product runs.
 int set_product_scatter(const float* match, float* const* out, int n, int cols);
 bool product_is_scattered(const float* out);
+// A tensor map over 16-bit elements: d0 contiguous, d1 columns ld elements apart, boxes of b0 x b1 swizzled by 128 bytes (b0 = 64).
+int gemm_path();      // b200_set_gemm_path
+bool tma_available();
+int take_injected_bytes();   // b200_test_inject_stage_bytes, for one product
+bool plane_map(CUtensorMap* out, const void* ptr, uint64_t d0, uint64_t d1, uint64_t ld, uint32_t b0, uint32_t b1);
 int gemm_simt(const GemmProblem& g);
 // fp32-grade products of any alignment in one launch (gemm_small.cu); ERROR_UNSUPPORTED for term lists that are
 // not whole products (scaled half-precision planes, single parts).

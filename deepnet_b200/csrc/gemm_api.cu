@@ -668,6 +668,7 @@ __global__ void k_update_scale(float* scale) {
 }  // namespace
 
 namespace b200 {
+int gemm_path() { return g_path; }
 int rewrite_f16_planes_if(const float* x, uint16_t* aux, int rows, long n, const float* exp_dev, const float* only_if) {
   if (n == 0) return 0;
   const bool svec = (rows % 4 == 0) && ((((uintptr_t)x) & 15) == 0);

@@ -153,3 +153,152 @@ def test_infinities_and_nan_stay_in_their_case(cm):
         keep = [c for c in range(N) if c not in (1, 3)]
         assert np.array_equal(got[:, keep], clean[:, keep])
         assert np.isnan(got[:, 1]).all() and not np.isfinite(got[:, 3]).all()
+
+
+def on_path(cm, path, call):
+    cm.set_gemm_path(path)
+    try:
+        return call()
+    finally:
+        cm.set_gemm_path(0)
+
+
+def columns_bound(w, x, k):
+    """`product_bound` for operands with a power of two a column: the magnitudes of w's and x's columns, whatever the others'."""
+    aw, ax = np.abs(w), np.abs(x)
+    return (k * U + 2.0 ** -18) * (aw.T @ ax) + 2.0 ** -30 * k * aw.max(0)[:, None] * ax.max(0)[None]
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("shape", SHAPES + [(64, 128, 256), (65, 129, 257), (40, 600, 33), (4096, 300, 70), (130, 5000, 600), (1000, 9, 3000)])
+def test_tensor_cores_and_cuda_cores_give_the_products(cm, shape, path):
+    """Either kernel at every size, over columns whose magnitudes lie up to 2^80 apart, with and without planes kept by the caller."""
+    V, H, N = shape
+    rng = np.random.default_rng(V * 5 + H * 3 + N)
+    wg, wu = (np.ldexp(rng.standard_normal((V, H)), rng.integers(-30, 10, (1, H))).astype(np.float32) for _ in range(2))
+    x = np.ldexp(rng.standard_normal((V, N)), rng.integers(-30, 10, (1, N))).astype(np.float32)
+    x[:, N // 2] = 0
+    wg[:, H // 3] = 0
+    ga, gb, gx = cm.CUDAMatrix(wg), cm.CUDAMatrix(wu), cm.CUDAMatrix(x)
+    gm, um, y, y2 = (cm.empty((H, N)) for _ in range(4))
+    on_path(cm, path, lambda: cm.gated_product(ga, gb, gx, y, activation="linear", gate=gm, up=um))
+    A, B, X = (v.astype(np.float64) for v in (wg, wu, x))
+    within(get(gm), A.T @ X, columns_bound(A, X, V) + 1e-37)
+    within(get(um), B.T @ X, columns_bound(B, X, V) + 1e-37)
+    within(get(y), get(gm).astype(np.float64) * get(um), U * np.abs(get(gm).astype(np.float64) * get(um)) + 1e-37)
+    planes = cm.GatedPlanes(ga, gb)
+    on_path(cm, path, lambda: cm.gated_product(ga, gb, gx, y2, activation="linear", planes=planes))
+    assert np.array_equal(get(y2), get(y))
+    other = cm.CUDAMatrix(wg[:, ::-1])                                      # filled again
+    planes.fill(other, gb)
+    on_path(cm, path, lambda: cm.gated_product(other, gb, gx, y2, activation="linear", gate=um, up=cm.empty((H, N)), planes=planes))
+    assert np.array_equal(get(um), get(gm)[::-1])
+    assert cm.read_status() == 0
+
+
+def test_extreme_magnitudes_on_tensor_cores(cm):
+    """Powers of two whose product is no normal number, and results at the ends of the range."""
+    rng = np.random.default_rng(21)
+    V, H, N = 200, 140, 40
+    w, x = rng.standard_normal((V, H)), rng.standard_normal((V, N))
+    for ew, ex in ((-70, -70), (60, 50), (-100, 100), (90, -110)):
+        a, b = np.ldexp(w, ew).astype(np.float32), np.ldexp(x, ex).astype(np.float32)
+        gm, um = cm.empty((H, N)), cm.empty((H, N))
+        on_path(cm, 1, lambda: cm.gated_product(cm.CUDAMatrix(a), cm.CUDAMatrix(a), cm.CUDAMatrix(b), activation="linear", gate=gm, up=um))
+        A, X = a.astype(np.float64), b.astype(np.float64)
+        within(get(gm), A.T @ X, columns_bound(A, X, V) + 2.0 ** -126)
+        assert np.array_equal(get(gm), get(um))
+    assert cm.read_status() == 0
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_matrices_that_start_anywhere(cm, off):
+    rng = np.random.default_rng(off)
+
+    def at(a):
+        big = cm.CUDAMatrix(np.concatenate([np.zeros(off, np.float32), np.asarray(a, np.float32).ravel(order="F")]).reshape(-1, 1))
+        v = big.slice(off, off + a.size)
+        v.reshape(a.shape)
+        return v
+    V, H, N = 256, 128, 96
+    wg, wu, x, dy = (rng.standard_normal(s).astype(np.float32) for s in ((V, H), (V, H), (V, N), (H, N)))
+    got = []
+    for place in (cm.CUDAMatrix, at):
+        m = [place(v) for v in (wg, wu, x, dy)]
+        gm, um, y, dx, dw = (place(np.zeros(s, np.float32)) for s in ((H, N), (H, N), (H, N), (V, N), (V, H)))
+        cm.gated_product(m[0], m[1], m[2], y, activation="silu", gate=gm, up=um)
+        first = [get(v) for v in (y, gm, um)]
+        cm.gated_product_deriv(m[3], gm, um, m[0], m[1], m[2], activation="silu", grad_x=dx, grad_up_w=dw)
+        got.append(first + [get(dx), get(dw)])
+    for a, b in zip(*got):          # the same sums by another kernel at most
+        size = np.abs(a).max()
+        np.testing.assert_allclose(a, b, rtol=0, atol=size * 2 * (256 * U + 2.0 ** -18) * 30)
+
+
+def test_a_wait_that_cannot_end_is_reported(cm):
+    """A product that is told to expect more bytes than its copies bring: the wait runs into its limit, the kernel returns, the status
+    word says so, and the next product works."""
+    rng = np.random.default_rng(4)
+    w, x = cm.CUDAMatrix(rng.standard_normal((512, 512)).astype(np.float32)), cm.CUDAMatrix(rng.standard_normal((512, 512)).astype(np.float32))
+    want = get(on_path(cm, 1, lambda: cm.gated_product(w, w, x)))
+    assert cm.read_status() == 0
+    cm.set_wait_limit(20000)                   # milliseconds
+    try:
+        cm._lib.b200_test_inject_stage_bytes(64)
+        on_path(cm, 1, lambda: cm.gated_product(w, w, x))
+        assert 31 <= cm.read_status() <= 34    # (waits until the kernel has returned)
+        assert cm.read_status() == 0
+    finally:
+        cm.set_wait_limit(0)
+    assert np.array_equal(get(on_path(cm, 1, lambda: cm.gated_product(w, w, x))), want)
+    assert cm.read_status() == 0
+
+
+class _On(object):
+    """The library's calls on a stream of torch's; with a graph, recorded."""
+
+    def __init__(self, cm, graph=None):
+        self.cm, self.stream, self.graph = cm, torch.cuda.Stream(), graph
+
+    def __enter__(self):
+        torch.cuda.synchronize()
+        self.cm._check(self.cm._lib.b200_set_stream(self.stream.cuda_stream))
+        if self.graph is not None:
+            self.ctx = torch.cuda.graph(self.graph, stream=self.stream)
+            self.ctx.__enter__()
+        return self
+
+    def __exit__(self, *e):
+        try:
+            if self.graph is not None:
+                self.ctx.__exit__(*e)
+        finally:
+            self.cm._lib.b200_set_stream(None)
+        torch.cuda.synchronize()
+
+
+def test_two_recorded_forward_passes_share_no_scratch(cm):
+    rng = np.random.default_rng(8)
+    torch.zeros(1, device="cuda")
+    sets, streams, graphs = [], [], [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    for V, H, N in ((700, 900, 300), (1300, 500, 200)):
+        s = [cm.CUDAMatrix(rng.standard_normal(shape).astype(np.float32)) for shape in ((V, H), (V, H), (V, N))] + [cm.empty((H, N))]
+        sets.append(s)
+    for s, graph in zip(sets, graphs):
+        with _On(cm, graph) as on:
+            cm.gated_product(*s, activation="gelu")
+        streams.append(on.stream)
+    want = []
+    for s in sets:
+        cm.gated_product(*s, activation="gelu")
+        want.append(get(s[3]))
+        s[3].assign(0)
+    cm.cuda_sync_threads()
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for s, w in zip(sets, want):
+        assert np.array_equal(get(s[3]), w)
+    assert cm.read_status() == 0

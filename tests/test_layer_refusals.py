@@ -98,8 +98,8 @@ def test_log_prob_deriv_refuses():
 
 
 def test_gated_product_refuses():
-    def f(wg, wu, x, bg=None, bu=None, act=1, gate=None, up=None, y=None):
-        return cm._lib.gated_product(wg, wu, x, bg, bu, ct.c_int(act), gate, up, y if y is not None else mat(7, 5))
+    def f(wg, wu, x, bg=None, bu=None, act=1, gate=None, up=None, y=None, planes=(None,) * 3):
+        return cm._lib.gated_product(wg, wu, x, bg, bu, ct.c_int(act), *planes, gate, up, y if y is not None else mat(7, 5))
     w, x = (lambda **k: mat(9, 7, **k)), (lambda **k: mat(9, 5, **k))
     assert f(w(), mat(9, 6), x()) == DIMENSIONS
     assert f(w(), w(), mat(8, 5)) == DIMENSIONS
@@ -112,6 +112,17 @@ def test_gated_product_refuses():
     assert f(w(), w(on_device=0), x()) == NOT_ON_DEVICE and f(w(), w(), x(), y=mat(7, 5, on_device=0)) == NOT_ON_DEVICE
     assert f(w(), w(), x(), act=-1) == UNSUPPORTED and f(w(), w(), x(), act=5) == UNSUPPORTED
     assert f(w(), w(), mat(9, 0), y=mat(7, 0)) == 0
+    # planes: all three, of the weights' shapes, on 16 bytes
+    good = lambda: [mat(16, 7), mat(16, 7), mat(2, 7)]
+    fill = lambda planes: cm._lib.gated_planes(w(), w(), *planes)
+    for i, bad, err in ((0, None, DIMENSIONS), (1, mat(9, 7), DIMENSIONS), (2, mat(7, 2), DIMENSIONS), (1, mat(16, 7, on_device=0), NOT_ON_DEVICE),
+                        (0, mat(16, 7, trans=1), TRANSPOSED)):
+        planes = good()
+        planes[i] = bad
+        assert f(w(), w(), x(), planes=planes) == err and (fill(planes) == err)
+    planes = good()
+    planes[1].contents.data_device = ct.cast(8, ct.POINTER(ct.c_float))
+    assert f(w(), w(), x(), planes=planes) == UNSUPPORTED and fill(planes) == UNSUPPORTED
     with pytest.raises(cm.CUDAMatException):
         cm._gated_activation("softmax")
 
