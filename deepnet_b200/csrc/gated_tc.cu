@@ -45,15 +45,21 @@ struct GatedParams {
   uint32_t stage_tx;                         // bytes that both CTAs' copies of a stage bring
 };
 
-__device__ __forceinline__ float act_of(int activation, float g) {
+template <int kAct>
+__device__ __forceinline__ void activate_times(float (&g)[8], const float (&u)[8]) {
   float slope;
+#pragma unroll
+  for (int i = 0; i < 8; i++) g[i] = activate<kAct>(g[i], slope) * u[i];
+}
+// g = act(g) * u
+__device__ __forceinline__ void activate_times(int activation, float (&g)[8], const float (&u)[8]) {
   switch (activation) {
-    case kLogistic: return activate<kLogistic>(g, slope);
-    case kRelu: return activate<kRelu>(g, slope);
-    case kSilu: return activate<kSilu>(g, slope);
-    case kGelu: return activate<kGelu>(g, slope);
+    case kLogistic: activate_times<kLogistic>(g, u); break;
+    case kRelu: activate_times<kRelu>(g, u); break;
+    case kSilu: activate_times<kSilu>(g, u); break;
+    case kGelu: activate_times<kGelu>(g, u); break;
+    default: activate_times<kLinear>(g, u);
   }
-  return g;
 }
 
 // v / (2^a 2^b) for the factors r = 2^-a, c = 2^-b: one product where theirs is a normal number.
@@ -222,11 +228,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kDrainRegs));
-    // Warp: lanes 32 q .. of the accumulator (q 0, 1 gate, 2, 3 up of units 32 (q & 1) ..), half the columns.
-    constexpr int kCols = T::kCols, kMine = kCols / 2, kRound = kMine < 16 ? kMine : 16;
-    const int ew = warp - 4, q = warp & 3, half = ew >> 2, which = q >> 1;
-    const uint32_t give = exchange + (uint32_t)(((q & 1) * 2 + half) * 8192 + which * 4096 + lane * 4);
-    const uint32_t take = exchange + (uint32_t)(((q & 1) * 2 + half) * 8192 + (1 - which) * 4096 + lane * 4);
+    // Warp: lanes 32 q .. of the accumulator (q 0, 1 gate, 2, 3 up of units 32 (q & 1) ..), half the columns.  The two warps that
+    // hold a unit's sums stage sixteen columns of both, then each finishes eight of them.  The code of a column is there once,
+    // not once a column: it runs seldom, and unrolled over the columns and the activations it would be fetched from memory each time.
+    constexpr int kCols = T::kCols, kLoad = kCols < 32 ? kCols : 32;
+    const int ew = warp - 4, q = warp & 3, half = ew >> 2, which = q >> 1, pair = (q & 1) * 2 + half;
+    const uint32_t stage_at = exchange + (uint32_t)(pair * 8192 + lane * 4);
     uint32_t chunk = 0;
     const int chunks = (k_iters + kChunk - 1) / kChunk;
     bool ok = true;
@@ -247,57 +254,65 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
         tc_fence_after();
         const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * kCols);
 #pragma unroll
-        for (int j = 0; j < kCols; j += 16) {
-          float v[16];
-          tmem_ld16(from + j, v);
+        for (int j = 0; j < kCols; j += kLoad) {
+          float v[kLoad];
+          if constexpr (kLoad == 32) tmem_ld32(from + j, v);
+          else tmem_ld16(from + j, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; i++) sum[j + i] += v[i];
+          for (int i = 0; i < kLoad; i++) sum[j + i] += v[i];
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_leader(free_(acc), 0);
       }
       // both warps of a pair go on, or neither: they wait for each other below
-      ok = all_ok(1 + (q & 1) * 2 + half, ok);
+      ok = all_ok(1 + pair, ok);
       if (!ok) break;
       const bool in = unit < p.M;
-      const float r = in ? p.w_inv[2L * unit + which] : 0.0f;
-      const float* b = which ? p.bu : p.bg;
-      const float bias = in && b ? b[unit] : 0.0f;
-      // the pair's first warp finishes the first half of the columns, its second the second
-      auto finish = [&](auto second) {
-        constexpr bool kSecond = decltype(second)::value;
+      const float2 r = in ? make_float2(p.w_inv[2L * unit], p.w_inv[2L * unit + 1]) : make_float2(0.0f, 0.0f);
+      const float bg = in && p.bg ? p.bg[unit] : 0.0f, bu = in && p.bu ? p.bu[unit] : 0.0f;
+      float *yo = p.y + unit, *go = p.gate + unit, *uo = p.up + unit;
+#pragma unroll 1
+      for (int round = 0; round < kCols / 16; round++) {
+        const uint32_t buf = stage_at + (uint32_t)(round & 1) * 4096u;
+        float c[8];
+        const int first_n = n0 + 16 * round + 8 * which;
 #pragma unroll
-        for (int j0 = 0, round = 0; j0 < kMine; j0 += kRound, round++) {
-          const uint32_t buf = (uint32_t)(round & 1) * 2048u;
+        for (int i = 0; i < 8; i++) c[i] = first_n + i < p.N ? __ldg(p.x_inv + first_n + i) : 1.0f;
 #pragma unroll
-          for (int i = 0; i < kRound; i++) {
-            const int j = (kSecond ? 0 : kMine) + j0 + i, n = n0 + j;
-            const float v = unscale(sum[j], r, n < p.N ? p.x_inv[n] : 1.0f) + bias;
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(give + buf + i * 128), "f"(v) : "memory");
+        for (int x = 0; x < kCols / 16; x++)
+          if (x == round) {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(buf + (uint32_t)which * 2048u + i * 128), "f"(sum[16 * x + i]));
           }
-          named_bar_sync(1 + (q & 1) * 2 + half, 64);
+        named_bar_sync(1 + pair, 64);
+        float gs[8], us[8];
 #pragma unroll
-          for (int i = 0; i < kRound; i++) {
-            const int j = (kSecond ? kMine : 0) + j0 + i, n = n0 + j;
-            float other;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(take + buf + i * 128) : "memory");
-            if (!in || n >= p.N) continue;
-            const float mine = unscale(sum[j], r, p.x_inv[n]) + bias;
-            const float g = kSecond ? other : mine, u = kSecond ? mine : other;
-            const long at = (long)n * p.M + unit;
-            if (p.gate) {
-              p.gate[at] = g;
-              p.up[at] = u;
-            }
-            p.y[at] = act_of(p.activation, g) * u;
-          }
+        for (int i = 0; i < 8; i++) {
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(gs[i]) : "r"(buf + (uint32_t)(8 * which + i) * 128u));
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(us[i]) : "r"(buf + 2048u + (uint32_t)(8 * which + i) * 128u));
         }
-        if (kMine / kRound % 2) named_bar_sync(1 + (q & 1) * 2 + half, 64);   // (the next tile starts with the buffer just read)
-      };
-      if (which) finish(std::integral_constant<bool, true>{});
-      else finish(std::integral_constant<bool, false>{});
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          gs[i] = unscale(gs[i], r.x, c[i]) + bg;
+          us[i] = unscale(us[i], r.y, c[i]) + bu;
+        }
+        const int live = in ? min(8, p.N - first_n) : 0;
+        if (p.gate) {
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (i < live) {
+              go[(long)(first_n + i) * p.M] = gs[i];
+              uo[(long)(first_n + i) * p.M] = us[i];
+            }
+        }
+        activate_times(p.activation, gs, us);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (i < live) yo[(long)(first_n + i) * p.M] = gs[i];
+      }
     }
   }
   tc_fence_before();
@@ -346,65 +361,98 @@ int launch(GatedParams& p) {
 // ---- matrices as planes --------------------------------------------------------------------
 struct SplitJobs {
   SplitJob job[3];
-  int first[4];          // blocks
-  int h, lda, per_block; // columns of a block: one (all its warps) or one a warp
-  bool vec[3];
+  int first[3];          // each one's first block: of eight columns, or of one
+  int h, lda;
 };
 
-// One column by `threads` threads: its largest finite magnitude, then the planes (the second read comes from L1 or L2).
-template <bool kBlock>
-__global__ void __launch_bounds__(256) k_split_columns(const SplitJobs a) {
+// A column's exponent from its largest finite magnitude (m: its bits), and its inverse scale written.
+__device__ __forceinline__ float scale_of(uint32_t m, float* inv) {
+  const int e = (int)f16_exponent(__uint_as_float(m));
+  if (inv) *inv = __int_as_float((127 - e) << 23);
+  return __int_as_float((127 + e) << 23);
+}
+__device__ __forceinline__ uint32_t magnitude(float v) {      // bits of finite magnitudes, in their order
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+template <int kVec>
+__device__ __forceinline__ void store_planes(uint16_t* lo, uint16_t* hi, long i, const float (&v)[kVec], float scale) {
+  uint16_t l[kVec], g[kVec];
+#pragma unroll
+  for (int j = 0; j < kVec; j++) split_f16(v[j], scale, l[j], g[j]);
+  if constexpr (kVec == 4) {
+    reinterpret_cast<ushort4*>(lo)[i] = make_ushort4(l[0], l[1], l[2], l[3]);
+    reinterpret_cast<ushort4*>(hi)[i] = make_ushort4(g[0], g[1], g[2], g[3]);
+  } else {
+    lo[i] = l[0];
+    hi[i] = g[0];
+  }
+}
+
+// A warp (or block) a column, which it holds in registers: kPer groups of kVec values a thread.  Bound by HBM: 8 bytes a value.
+template <int kVec, int kPer, bool kBlock>
+__global__ void __launch_bounds__(256) k_split_columns(const __grid_constant__ SplitJobs a) {
   __shared__ uint32_t red[8];
   grid_dependents_launch();
   grid_dependency_wait();
   const int which = blockIdx.x >= a.first[2] ? 2 : blockIdx.x >= a.first[1] ? 1 : 0;
-  const SplitJob j = a.job[which];
-  const int threads = kBlock ? 256 : 32, t = kBlock ? threadIdx.x : threadIdx.x & 31, h = a.h;
-  const long c = (long)(blockIdx.x - a.first[which]) * (kBlock ? 1 : 8) + (kBlock ? 0 : threadIdx.x >> 5);
-  if (c >= j.cols) return;
-  const float* x = j.x + c * h;
-  const bool vec = a.vec[which];
-  uint32_t m = 0;                                     // bits of a magnitude: in the magnitudes' order
-  auto see = [&](float v) {
-    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-    if (b < 0x7f800000u) m = max(m, b);
-  };
-  if (vec) {
-#pragma unroll 4
-    for (int i = t; i < h / 4; i += threads) {
-      const float4 v = reinterpret_cast<const float4*>(x)[i];
-      see(v.x); see(v.y); see(v.z); see(v.w);
+  const float* src = which == 2 ? a.job[2].x : which ? a.job[1].x : a.job[0].x;
+  uint16_t* planes = which == 2 ? a.job[2].planes : which ? a.job[1].planes : a.job[0].planes;
+  float* inv = which == 2 ? a.job[2].inv : which ? a.job[1].inv : a.job[0].inv;
+  const int stride = which == 2 ? a.job[2].inv_stride : which ? a.job[1].inv_stride : a.job[0].inv_stride;
+  const int cols = which == 2 ? a.job[2].cols : which ? a.job[1].cols : a.job[0].cols;
+  const int at = blockIdx.x - (which == 2 ? a.first[2] : which ? a.first[1] : a.first[0]);
+  const int threads = kBlock ? 256 : 32, t = kBlock ? threadIdx.x : threadIdx.x & 31, items = a.h / kVec;
+  const long c = (long)at * (kBlock ? 1 : 8) + (kBlock ? 0 : threadIdx.x >> 5);
+  if (c >= cols) return;
+  const float* x = src + c * a.h;
+  float v[kPer][kVec];
+  uint32_t m = 0;
+  auto load = [&](int i, float (&to)[kVec]) {
+    if constexpr (kVec == 4) {
+      const float4 f = reinterpret_cast<const float4*>(x)[i];
+      to[0] = f.x; to[1] = f.y; to[2] = f.z; to[3] = f.w;
+    } else {
+      to[0] = x[i];
     }
-  } else {
-#pragma unroll 8
-    for (int i = t; i < h; i += threads) see(x[i]);
+  };
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    if (t + i * threads < items) {
+      load(t + i * threads, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; j++) v[i][j] = 0.0f;
+    }
   }
+#pragma unroll
+  for (int i = 0; i < kPer; i++)
+#pragma unroll
+    for (int j = 0; j < kVec; j++) m = max(m, magnitude(v[i][j]));
+  if (kBlock)        // (columns longer than that are read again below)
+    for (int i = t + kPer * threads; i < items; i += threads) {
+      float w[kVec];
+      load(i, w);
+#pragma unroll
+      for (int j = 0; j < kVec; j++) m = max(m, magnitude(w[j]));
+    }
   m = __reduce_max_sync(0xffffffffu, m);
   if (kBlock) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
     __syncthreads();
     m = __reduce_max_sync(0xffffffffu, red[threadIdx.x & 7]);
   }
-  const int e = (int)f16_exponent(__uint_as_float(m));
-  const float scale = __int_as_float((127 + e) << 23);
-  if (t == 0) j.inv[c * j.inv_stride] = __int_as_float((127 - e) << 23);
-  uint16_t *lo = j.planes + c * 2 * a.lda, *hi = lo + a.lda;
-  if (vec) {
-#pragma unroll 4
-    for (int i = t; i < h / 4; i += threads) {
-      const float4 v = reinterpret_cast<const float4*>(x)[i];
-      ushort4 l, g;
-      split_f16(v.x, scale, l.x, g.x);
-      split_f16(v.y, scale, l.y, g.y);
-      split_f16(v.z, scale, l.z, g.z);
-      split_f16(v.w, scale, l.w, g.w);
-      reinterpret_cast<ushort4*>(lo)[i] = l;
-      reinterpret_cast<ushort4*>(hi)[i] = g;
+  const float scale = scale_of(m, t == 0 ? inv + c * stride : nullptr);
+  uint16_t *lo = planes + c * 2 * a.lda, *hi = lo + a.lda;
+#pragma unroll
+  for (int i = 0; i < kPer; i++)
+    if (t + i * threads < items) store_planes<kVec>(lo, hi, t + i * threads, v[i], scale);
+  if (kBlock)
+    for (int i = t + kPer * threads; i < items; i += threads) {
+      float w[kVec];
+      load(i, w);
+      store_planes<kVec>(lo, hi, i, w, scale);
     }
-  } else {
-#pragma unroll 4
-    for (int i = t; i < h; i += threads) split_f16(x[i], scale, lo[i], hi[i]);
-  }
 }
 
 }  // namespace
@@ -413,19 +461,31 @@ int split_columns(const SplitJob* jobs, int njobs, int rows) {
   SplitJobs a = {};
   a.h = rows;
   a.lda = aux_rows(rows);
-  const bool block = rows > 1024;
+  bool vec = rows % 4 == 0;
+  for (int i = 0; i < njobs; i++) vec = vec && ((uintptr_t)jobs[i].x & 15) == 0;
+  const int items = vec ? rows / 4 : rows;
+  const bool block = items > 32 * 16;
   int at = 0;
   for (int i = 0; i < 3; i++) {
     a.first[i] = at;
     if (i >= njobs) continue;
     a.job[i] = jobs[i];
-    a.vec[i] = rows % 4 == 0 && ((uintptr_t)jobs[i].x & 15) == 0;
     at += block ? jobs[i].cols : (jobs[i].cols + 7) / 8;
   }
-  a.first[3] = at;
   if (at == 0) return 0;
-  if (block) (void)launch_dependent(k_split_columns<true>, dim3(at), dim3(256), 0, stream(), a);
-  else (void)launch_dependent(k_split_columns<false>, dim3(at), dim3(256), 0, stream(), a);
+#define SPLIT(VEC, PER, BLOCK) (void)launch_dependent(k_split_columns<VEC, PER, BLOCK>, dim3(at), dim3(256), 0, stream(), a)
+#define SPLIT_PER(PER, BLOCK)          \
+  do {                                 \
+    if (vec) SPLIT(4, PER, BLOCK);     \
+    else SPLIT(1, PER, BLOCK);         \
+  } while (0)
+  if (items <= 32 * 4) SPLIT_PER(4, false);
+  else if (items <= 32 * 8) SPLIT_PER(8, false);
+  else if (items <= 32 * 16) SPLIT_PER(16, false);
+  else if (items <= 256 * 4) SPLIT_PER(4, true);
+  else SPLIT_PER(8, true);
+#undef SPLIT_PER
+#undef SPLIT
   return check_launch();
 }
 
