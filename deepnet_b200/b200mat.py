@@ -918,6 +918,10 @@ class GatedPlanes(object):
         return self
 
 
+def _planes(planes):
+    return (planes.gate.p_mat, planes.up.p_mat, planes.scales.p_mat) if planes is not None else (None, None, None)
+
+
 def gated_product(gate_w, up_w, mat, target=None, activation="logistic", gate_bias=None, up_bias=None, gate=None, up=None, planes=None):
     """target = act(gate_w' mat + gate_bias) * (up_w' mat + up_bias) in one kernel: a gated layer's forward pass.  Weights are inputs x
     units, mat inputs x cases; activation one of `GATED_ACTIVATIONS` (silu: g logistic(g), gelu: g Phi(g)).  gate and up (units x
@@ -926,17 +930,16 @@ def gated_product(gate_w, up_w, mat, target=None, activation="logistic", gate_bi
     if target is None:
         target = empty((gate_w.shape[1], mat.shape[1]))
     _check(_lib.gated_product(gate_w.p_mat, up_w.p_mat, mat.p_mat, _p(gate_bias), _p(up_bias), _gated_activation(activation),
-                              *((m.p_mat for m in (planes.gate, planes.up, planes.scales)) if planes is not None else (None,) * 3),
-                              _p(gate), _p(up), target.p_mat))
+                              *_planes(planes), _p(gate), _p(up), target.p_mat))
     return target
 
 
 def gated_product_deriv(deriv, gate, up, gate_w, up_w, mat, activation="logistic", grad_x=None, grad_gate_w=None, grad_up_w=None,
-                        grad_gate_bias=None, grad_up_bias=None):
+                        grad_gate_bias=None, grad_up_bias=None, planes=None):
     """deriv is the gradient of `gated_product`'s target.  gate and up, as that call left them, are overwritten with their gradients;
-    the gradients of mat, weights and biases go to the matrices given for them."""
+    the gradients of mat, weights and biases go to the matrices given for them.  planes: the weights' `GatedPlanes`."""
     _check(_lib.gated_product_deriv(deriv.p_mat, gate.p_mat, up.p_mat, gate_w.p_mat, up_w.p_mat, mat.p_mat, _gated_activation(activation),
-                                    _p(grad_x), _p(grad_gate_w), _p(grad_up_w), _p(grad_gate_bias), _p(grad_up_bias)))
+                                    *_planes(planes), _p(grad_x), _p(grad_gate_w), _p(grad_up_w), _p(grad_gate_bias), _p(grad_up_bias)))
 
 
 def _build_bias_layers(layers, sq_acc):

@@ -9,7 +9,6 @@ using namespace b200;
 
 extern "C" {
 int dot(cudamat* mat1, cudamat* mat2, cudamat* target, float beta, float alpha);
-int sum_by_axis(cudamat* mat, cudamat* target, int axis);
 }
 
 namespace {
@@ -66,30 +65,173 @@ __global__ void __launch_bounds__(256) k_gated_simt(const GatedArgs a) {
     }
 }
 
-// gate, up = dG, dU
-template <int kAct, bool kVec>
-__global__ void __launch_bounds__(256) k_gated_deriv(const float* dy, float* gate, float* up, long n) {
+// ---- the derivative's elementwise part ------------------------------------------------------
+// A thread takes kVec units of some cases, one case after another: the units' sums and maxima stay in registers.  Bound by HBM:
+// 20 bytes a unit and case for the gradients, 8 + 16 for their planes.
+constexpr int kMostCases = 64, kDerivThreads = 128;
+
+template <int kVec>
+__device__ __forceinline__ void load(const float* p, float (&v)[kVec]) {
+  if constexpr (kVec == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  } else {
+    v[0] = *p;
+  }
+}
+template <int kVec>
+__device__ __forceinline__ void store(float* p, const float (&v)[kVec]) {
+  if constexpr (kVec == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else *p = v[0];
+}
+__device__ __forceinline__ uint32_t magnitude(float v) {      // bits of finite magnitudes, in their order
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// *p = max(*p, v), which is the same in any order.  Most blocks come too late to raise it: a look first (1024 x 1024 units and cases:
+// 83 us of the derivative without).
+__device__ __forceinline__ void raise(uint32_t* p, uint32_t v) {
+  if (v > *(volatile uint32_t*)p) atomicMax(p, v);
+}
+
+template <int kAct, int kVec>
+__global__ void __launch_bounds__(kDerivThreads) k_gated_deriv(const GatedDeriv a) {
   grid_dependents_launch();
   grid_dependency_wait();
-  const long step = (long)gridDim.x * blockDim.x;
-  auto one = [](float d, float& g, float& u) {
-    float slope;
-    const float act = activate<kAct>(g, slope);
-    g = d * u * slope;
-    u = d * act;
-  };
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < (kVec ? n / 4 : n); i += step) {
-    if (kVec) {
-      const float4 d = reinterpret_cast<const float4*>(dy)[i];
-      float4 g = reinterpret_cast<float4*>(gate)[i], u = reinterpret_cast<float4*>(up)[i];
-      one(d.x, g.x, u.x);
-      one(d.y, g.y, u.y);
-      one(d.z, g.z, u.z);
-      one(d.w, g.w, u.w);
-      reinterpret_cast<float4*>(gate)[i] = g;
-      reinterpret_cast<float4*>(up)[i] = u;
-    } else {
-      one(dy[i], gate[i], up[i]);
+  const int blocks_u = (a.H + kDerivThreads * kVec - 1) / (kDerivThreads * kVec), ub = blockIdx.x % blocks_u, cb = blockIdx.x / blocks_u;
+  const int r = (ub * kDerivThreads + threadIdx.x) * kVec;
+  const bool in = r < a.H;
+  const int c1 = min(a.N, (cb + 1) * a.cases);
+  float sg[kVec] = {}, su[kVec] = {}, wg[kVec], wu[kVec];
+  uint32_t mg[kVec] = {}, mu[kVec] = {};
+#pragma unroll
+  for (int j = 0; j < kVec; j++) {
+    wg[j] = in && a.w_inv ? a.w_inv[2L * (r + j)] : 0.0f;
+    wu[j] = in && a.w_inv ? a.w_inv[2L * (r + j) + 1] : 0.0f;
+  }
+#pragma unroll 2
+  for (int c = cb * a.cases; c < c1; c++) {
+    const long at = (long)c * a.H + r;
+    float d[kVec] = {}, g[kVec] = {}, u[kVec] = {};
+    if (in) {
+      load<kVec>(a.dy + at, d);
+      load<kVec>(a.gate + at, g);
+      load<kVec>(a.up + at, u);
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; j++) {
+      float slope;
+      const float act = activate<kAct>(g[j], slope);
+      g[j] = d[j] * u[j] * slope;
+      u[j] = d[j] * act;
+      sg[j] += g[j];
+      su[j] += u[j];
+    }
+    if (in) {
+      store<kVec>(a.gate + at, g);
+      store<kVec>(a.up + at, u);
+    }
+    if (a.token_max) {
+      const float xi = a.x_inv[c];
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < kVec; j++) {
+        m = max(m, max(magnitude(g[j] * wg[j]), magnitude(u[j] * wu[j])));
+        mg[j] = max(mg[j], magnitude(g[j] * xi));
+        mu[j] = max(mu[j], magnitude(u[j] * xi));
+      }
+      m = __reduce_max_sync(0xffffffffu, m);
+      if ((threadIdx.x & 31) == 0) raise(a.token_max + c, m);
+    }
+  }
+  if (!in) return;
+#pragma unroll
+  for (int j = 0; j < kVec; j++) {
+    if (a.part) {
+      a.part[2L * cb * a.H + r + j] = sg[j];
+      a.part[(2L * cb + 1) * a.H + r + j] = su[j];
+    }
+    if (a.token_max) {
+      raise(a.unit_max + 2L * (r + j), mg[j]);
+      raise(a.unit_max + 2L * (r + j) + 1, mu[j]);
+    }
+  }
+}
+
+// The blocks' sums, in order: 32 values a block, eight threads a value.
+__global__ void __launch_bounds__(256) k_gated_biases(const float* part, int blocks, float* dbg, float* dbu, int h) {
+  __shared__ float red[8][33];
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const long v = (long)blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (v < 2L * h) {
+#pragma unroll 8
+    for (int b = wid; b < blocks; b += 8) s += part[2L * b * h + v];
+  }
+  red[wid][lane] = s;
+  __syncthreads();
+  if (wid || v >= 2L * h) return;
+#pragma unroll
+  for (int k = 1; k < 8; k++) s += red[k][lane];
+  if (v < h) {
+    if (dbg) dbg[v] = s;
+  } else if (dbu) {
+    dbu[v - h] = s;
+  }
+}
+
+__device__ __forceinline__ float power_of(uint32_t max_bits, float* inv) {
+  const int e = (int)f16_exponent(__uint_as_float(max_bits));
+  if (inv) *inv = __int_as_float((127 - e) << 23);
+  return __int_as_float((127 + e) << 23);
+}
+
+template <int kVec>
+__global__ void __launch_bounds__(kDerivThreads) k_gradient_planes(const GradientPlanes a) {
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int blocks_u = (a.H + kDerivThreads * kVec - 1) / (kDerivThreads * kVec), ub = blockIdx.x % blocks_u, cb = blockIdx.x / blocks_u;
+  const int r = (ub * kDerivThreads + threadIdx.x) * kVec, lda = aux_rows(a.H);
+  if (r >= a.H) return;
+  const int c1 = min(a.N, (cb + 1) * a.cases);
+  float w[2][kVec], s[2][kVec];
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+#pragma unroll
+    for (int j = 0; j < kVec; j++) {
+      const long i = 2L * (r + j) + k;
+      w[k][j] = a.w_inv[i];
+      s[k][j] = power_of(a.unit_max[i], cb == 0 && a.by_unit[0] ? a.unit_inv + i : nullptr);
+    }
+#pragma unroll 2
+  for (int c = cb * a.cases; c < c1; c++) {
+    const float xi = a.x_inv[c], sc = power_of(a.token_max[c], r == 0 && a.by_case[0] ? a.case_inv + c : nullptr);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      float v[kVec];
+      load<kVec>((k ? a.up : a.gate) + (long)c * a.H + r, v);
+      auto write = [&](uint16_t* planes, const float (&f)[kVec], const float (&scale)[kVec]) {
+        uint16_t lo[kVec], hi[kVec], *at = planes + (long)c * 2 * lda + r;
+#pragma unroll
+        for (int j = 0; j < kVec; j++) split_f16(v[j] * f[j], scale[j], lo[j], hi[j]);
+        if constexpr (kVec == 4) {
+          *reinterpret_cast<ushort4*>(at) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<ushort4*>(at + lda) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+        } else {
+          at[0] = lo[0];
+          at[lda] = hi[0];
+        }
+      };
+      float one[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; j++) one[j] = sc;
+      if (a.by_case[0]) write(a.by_case[k], w[k], one);
+#pragma unroll
+      for (int j = 0; j < kVec; j++) one[j] = xi;
+      if (a.by_unit[0]) write(a.by_unit[k], one, s[k]);
     }
   }
 }
@@ -101,6 +243,7 @@ int bias_ok(const cudamat* v, int h) {
   return numel(v) == h && (v->size[0] == 1 || v->size[1] == 1) ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
 }
 bool is(const cudamat* m, int rows, int cols) { return m->size[0] == rows && m->size[1] == cols; }
+constexpr long kTensorDerivWork = 1L << 40;
 constexpr long kTensorWork = 1L << 21;      // multiply-adds of one of the products from which the tensor cores take both
 int weights_ok(const cudamat* gate_w, const cudamat* up_w) {
   if (!gate_w->on_device || !up_w->on_device) return ERROR_NOT_ON_DEVICE;
@@ -122,6 +265,39 @@ int planes_ok(const cudamat* w, const cudamat* gate_planes, const cudamat* up_pl
 }
 
 }  // namespace
+
+namespace b200 {
+// As many as leave the device some blocks an SM (of 512 units each), 4 to kMostCases.
+int gated_deriv_cases(int H, int N) {
+  const long cases = (long)((H + 511) / 512) * N / (8L * sm_count());
+  return cases < 4 ? 4 : cases > kMostCases ? kMostCases : (int)cases;
+}
+static long deriv_grid(int H, int N, int cases, bool vec) {
+  const int units = kDerivThreads * (vec ? 4 : 1);
+  return (long)((N + cases - 1) / cases) * ((H + units - 1) / units);
+}
+int gated_deriv(const GatedDeriv& d) {
+  const bool vec = d.H % 4 == 0 && on16(d.dy) && on16(d.gate) && on16(d.up);
+  const long blocks = deriv_grid(d.H, d.N, d.cases, vec);
+  if (blocks > 0x7fffffffL) return ERROR_UNSUPPORTED;
+#define DERIV(ACT)                                                                                                  \
+  case ACT:                                                                                                         \
+    if (vec) (void)launch_dependent(k_gated_deriv<ACT, 4>, dim3((unsigned)blocks), dim3(kDerivThreads), 0, stream(), d);       \
+    else (void)launch_dependent(k_gated_deriv<ACT, 1>, dim3((unsigned)blocks), dim3(kDerivThreads), 0, stream(), d);           \
+    break
+  switch (d.activation) { DERIV(kLinear); DERIV(kLogistic); DERIV(kRelu); DERIV(kSilu); DERIV(kGelu); }
+#undef DERIV
+  return check_launch();
+}
+int gradient_planes(const GradientPlanes& g) {
+  const bool vec = g.H % 4 == 0 && on16(g.gate) && on16(g.up);
+  const long blocks = deriv_grid(g.H, g.N, g.cases, vec);
+  if (blocks > 0x7fffffffL) return ERROR_UNSUPPORTED;
+  if (vec) (void)launch_dependent(k_gradient_planes<4>, dim3((unsigned)blocks), dim3(kDerivThreads), 0, stream(), g);
+  else (void)launch_dependent(k_gradient_planes<1>, dim3((unsigned)blocks), dim3(kDerivThreads), 0, stream(), g);
+  return check_launch();
+}
+}  // namespace b200
 
 extern "C" {
 
@@ -193,9 +369,10 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
 }
 
 int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gate_w, cudamat* up_w, cudamat* mat, int activation,
-                        cudamat* grad_mat, cudamat* grad_gate_w, cudamat* grad_up_w, cudamat* grad_gate_bias, cudamat* grad_up_bias) {
+                        cudamat* gate_planes, cudamat* up_planes, cudamat* scales, cudamat* grad_mat, cudamat* grad_gate_w, cudamat* grad_up_w, cudamat* grad_gate_bias, cudamat* grad_up_bias) {
   int err = weights_ok(gate_w, up_w);
   if (err) return err;
+  if ((gate_planes || up_planes || scales) && (err = planes_ok(gate_w, gate_planes, up_planes, scales))) return err;
   const int V = gate_w->size[0], H = gate_w->size[1], N = mat->size[1];
   struct { cudamat* m; int rows, cols; } want[] = {{deriv, H, N}, {gate, H, N}, {up, H, N}, {mat, V, N}, {grad_mat, V, N},
                                                    {grad_gate_w, V, H}, {grad_up_w, V, H}};
@@ -210,37 +387,123 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     set_error("no such activation");
     return ERROR_UNSUPPORTED;
   }
-  const long n = (long)H * N;
-  if (N == 0 && H > 0) {            // sums over no cases
-    for (cudamat* m : {grad_gate_bias, grad_up_bias})
-      if (m && cudaMemsetAsync(m->data_device, 0, sizeof(float) * H, stream()) != cudaSuccess)
+  if (N == 0 || H == 0) {           // sums over no cases, or no units
+    for (cudamat* m : {grad_gate_bias, grad_up_bias, grad_gate_w, grad_up_w, grad_mat})
+      if (m && numel(m) && cudaMemsetAsync(m->data_device, 0, sizeof(float) * numel(m), stream()) != cudaSuccess)
         return set_error(cudaGetErrorString(cudaGetLastError()));
+    return 0;
   }
-  if (n > 0) {
-    const float* dy = deriv->data_device;
-    float *g = gate->data_device, *u = up->data_device;
-    const bool vec = n % 4 == 0 && on16(dy) && on16(g) && on16(u);
-    long blocks = ((vec ? n / 4 : n) + 255) / 256;
-    if (blocks > 16L * sm_count()) blocks = 16L * sm_count();
-#define DERIV(ACT)                                                                                                               \
-  case ACT:                                                                                                                      \
-    if (vec) (void)launch_dependent(k_gated_deriv<ACT, true>, dim3((unsigned)blocks), dim3(256), 0, stream(), dy, g, u, n);       \
-    else (void)launch_dependent(k_gated_deriv<ACT, false>, dim3((unsigned)blocks), dim3(256), 0, stream(), dy, g, u, n);          \
-    break
-    switch (activation) { DERIV(kLinear); DERIV(kLogistic); DERIV(kRelu); DERIV(kSilu); DERIV(kGelu); }
-#undef DERIV
+  const bool biases = grad_gate_bias || grad_up_bias, weights = grad_gate_w || grad_up_w;
+  const bool large = (long)V * H * N >= kTensorDerivWork;
+  const bool tc = V > 0 && (weights || grad_mat) && gemm_path() != 2 && (large || gemm_path() == 1) && tma_available();
+  const int cases = gated_deriv_cases(H, N), blocks = (N + cases - 1) / cases;
+  const bool split_w = tc && !gate_planes;
+  // scratch, each part on 256 bytes
+  size_t room_bytes = 0;
+  auto take = [&](bool wanted, size_t bytes) {
+    const size_t at = room_bytes;
+    if (wanted) room_bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  const size_t unit = sizeof(float) * 2 * (size_t)H, each = sizeof(float) * (size_t)N, hn = (size_t)aux_rows(H) * N * 4;
+  const size_t at_part = take(biases, unit * blocks), at_tmax = take(tc, each), at_umax = take(tc, unit), after_max = room_bytes;
+  const size_t at_xi = take(tc, each), at_wi = take(split_w, unit), at_ci = take(tc, each), at_ui = take(tc, unit);
+  const size_t at_x = take(tc, (size_t)aux_rows(V) * N * 4), vh = (size_t)aux_rows(V) * H * 4, at_wg = take(split_w, vh), at_wu = take(split_w, vh);
+  const size_t at_cg = take(tc && grad_mat, hn), at_cu = take(tc && grad_mat, hn), at_ug = take(tc && weights, hn), at_uu = take(tc && weights, hn);
+  CallScratch room(6, room_bytes);
+  char* const p = (char*)room.p;
+  if (room_bytes && !p) return CUDA_ERROR;
+  GatedDeriv d = {};
+  d.dy = deriv->data_device;
+  d.gate = gate->data_device;
+  d.up = up->data_device;
+  d.H = H;
+  d.N = N;
+  d.activation = activation;
+  d.cases = cases;
+  d.part = biases ? (float*)(p + at_part) : nullptr;
+  Planes xp = {}, wgp = {}, wup = {};
+  if (tc) {
+    d.token_max = (uint32_t*)(p + at_tmax);
+    d.unit_max = (uint32_t*)(p + at_umax);
+    d.x_inv = (float*)(p + at_xi);
+    d.w_inv = split_w ? (float*)(p + at_wi) : scales->data_device;
+    xp = {(uint16_t*)(p + at_x), V, N};
+    wgp = {split_w ? (uint16_t*)(p + at_wg) : (uint16_t*)gate_planes->data_device, V, H};
+    wup = {split_w ? (uint16_t*)(p + at_wu) : (uint16_t*)up_planes->data_device, V, H};
+    const SplitJob jobs[3] = {{mat->data_device, (uint16_t*)xp.p, (float*)d.x_inv, 1, N},
+                              {gate_w->data_device, (uint16_t*)wgp.p, (float*)d.w_inv, 2, H},
+                              {up_w->data_device, (uint16_t*)wup.p, (float*)d.w_inv + 1, 2, H}};
+    if (cudaMemsetAsync(p + at_tmax, 0, after_max - at_tmax, stream()) != cudaSuccess)
+      return set_error(cudaGetErrorString(cudaGetLastError()));
+    if ((err = split_columns(jobs, split_w ? 3 : 1, V))) return err;
+  }
+  if ((err = gated_deriv(d))) return err;
+  if (biases) {
+    (void)launch_dependent(k_gated_biases, dim3((2 * (unsigned)H + 31) / 32), dim3(256), 0, stream(), d.part, blocks,
+                           grad_gate_bias ? grad_gate_bias->data_device : nullptr, grad_up_bias ? grad_up_bias->data_device : nullptr, H);
     if ((err = check_launch())) return err;
   }
-  if (grad_gate_bias && n && (err = sum_by_axis(gate, grad_gate_bias, 1))) return err;
-  if (grad_up_bias && n && (err = sum_by_axis(up, grad_up_bias, 1))) return err;
-  cudamat dg = *gate, du = *up;
-  dg.is_trans = du.is_trans = 1;
-  dg.owns_data = du.owns_data = 0;
-  if (grad_gate_w && (err = dot(mat, &dg, grad_gate_w, 0.0f, 1.0f))) return err;
-  if (grad_up_w && (err = dot(mat, &du, grad_up_w, 0.0f, 1.0f))) return err;
+  if (!tc) {
+    cudamat dg = *gate, du = *up;
+    dg.is_trans = du.is_trans = 1;
+    dg.owns_data = du.owns_data = 0;
+    if (grad_gate_w && V && (err = dot(mat, &dg, grad_gate_w, 0.0f, 1.0f))) return err;
+    if (grad_up_w && V && (err = dot(mat, &du, grad_up_w, 0.0f, 1.0f))) return err;
+    if (grad_mat && V) {
+      if ((err = dot(gate_w, gate, grad_mat, 0.0f, 1.0f))) return err;
+      if ((err = dot(up_w, up, grad_mat, 1.0f, 1.0f))) return err;
+    }
+    return 0;
+  }
+  GradientPlanes g = {};
+  g.cases = cases;
+  g.gate = d.gate;
+  g.up = d.up;
+  g.H = H;
+  g.N = N;
+  g.w_inv = d.w_inv;
+  g.x_inv = d.x_inv;
+  g.token_max = d.token_max;
+  g.unit_max = d.unit_max;
+  g.case_inv = (float*)(p + at_ci);
+  g.unit_inv = (float*)(p + at_ui);
   if (grad_mat) {
-    if ((err = dot(gate_w, gate, grad_mat, 0.0f, 1.0f))) return err;
-    if ((err = dot(up_w, up, grad_mat, 1.0f, 1.0f))) return err;
+    g.by_case[0] = (uint16_t*)(p + at_cg);
+    g.by_case[1] = (uint16_t*)(p + at_cu);
+  }
+  if (weights) {
+    g.by_unit[0] = (uint16_t*)(p + at_ug);
+    g.by_unit[1] = (uint16_t*)(p + at_uu);
+  }
+  if ((err = gradient_planes(g))) return err;
+  if (grad_mat) {
+    PlaneProduct f = {};
+    f.npairs = 2;
+    f.a[0] = wgp;
+    f.a[1] = wup;
+    f.b[0] = {g.by_case[0], H, N};
+    f.b[1] = {g.by_case[1], H, N};
+    f.nout = 1;
+    f.out[0] = grad_mat->data_device;
+    f.inv[0] = g.case_inv;
+    f.inv_stride = 1;
+    if ((err = plane_product(f))) return err;
+  }
+  if (weights) {
+    PlaneProduct f = {};
+    f.npairs = 1;
+    f.trans = true;
+    f.a[0] = xp;
+    f.inv_stride = 2;
+    cudamat* const out[2] = {grad_gate_w, grad_up_w};
+    for (int k = 0; k < 2; k++) {
+      if (!out[k]) continue;
+      f.b[f.nout] = {g.by_unit[k], H, N};
+      f.out[f.nout] = out[k]->data_device;
+      f.inv[f.nout++] = g.unit_inv + k;
+    }
+    if ((err = plane_product(f))) return err;
   }
   return 0;
 }

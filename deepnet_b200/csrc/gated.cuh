@@ -54,4 +54,45 @@ struct GatedForward {
 };
 int gated_tc(const GatedForward& f);
 
+// out[:, n] = inv(n) sum over the pairs (a, b) of a . op(b): planes of a as stored (their rows are the output's), of b as stored
+// (its columns are the output's, `trans` false, up to two pairs) or transposed (its rows are; one pair, and with a second b a second
+// out, for the same a).
+struct PlaneProduct {
+  int npairs;
+  Planes a[2], b[2];
+  bool trans;
+  int nout;
+  float* out[2];
+  const float* inv[2];      // of out's columns; stride inv_stride
+  int inv_stride;
+};
+int plane_product(const PlaneProduct& f);
+
+// gate, up = their gradients dG, dU from dy; with `maxima` the largest |dG| w_inv, |dU| w_inv of each case (token_max) and the largest
+// |dG| x_inv, |dU| x_inv of each unit (unit_max, gate's and up's): bits of floats, all zero before.  part: sums of dG and dU over the
+// cases of a block, blocks of `cases` x 2 x H, or null.
+struct GatedDeriv {
+  const float* dy;
+  float *gate, *up;
+  int H, N, activation;
+  const float *w_inv, *x_inv;
+  uint32_t *token_max, *unit_max;
+  float* part;
+  int cases;                // of a block
+};
+int gated_deriv_cases(int H, int N);
+int gated_deriv(const GatedDeriv& d);
+// dG and dU as planes: with the weights' scales divided out and one of their own a case (by_case: gate's, up's; inverses case_inv),
+// and with the inputs' scales divided out and one of their own a unit (by_unit; unit_inv 2 x H).  Either may be null.
+struct GradientPlanes {
+  const float *gate, *up;
+  int H, N;
+  const float *w_inv, *x_inv;
+  const uint32_t *token_max, *unit_max;
+  uint16_t *by_case[2], *by_unit[2];
+  float *case_inv, *unit_inv;
+  int cases;
+};
+int gradient_planes(const GradientPlanes& g);
+
 }  // namespace b200

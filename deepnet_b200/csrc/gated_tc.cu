@@ -14,7 +14,6 @@
 // bounded; on expiry the kernel records a status word, drains and returns.
 #include <cuda.h>
 
-#include <mutex>
 #include <type_traits>
 
 #include "gated.cuh"
@@ -324,25 +323,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
   }
 }
 
-template <int BN>
-int launch(GatedParams& p) {
-  static std::mutex mu;
-  static bool ready[64] = {false};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_error("cudaGetDevice failed");
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!ready[dev] && cudaFuncSetAttribute(k_gated_tc<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-      return set_error("cudaFuncSetAttribute(max dynamic shared memory) failed");
-    ready[dev] = true;
-  }
-  p.stage_tx = 2 * Tile<BN>::kStageBytes + (uint32_t)take_injected_bytes();
-  const int tiles = p.tiles_m * p.tiles_n;
-  int pairs = sm_count() / 2;
+// Pairs of CTAs for `tiles` tiles.
+template <class Params>
+int launch_pairs(void (*kernel)(Params), const Params& p, long tiles) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+    return set_error("cudaFuncSetAttribute(max dynamic shared memory) failed");
+  long pairs = sm_count() / 2;
   if (pairs > tiles) pairs = tiles;
   if (pairs < 1) pairs = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * pairs);
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream();
@@ -354,8 +344,212 @@ int launch(GatedParams& p) {
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = dependent_launch_enabled() ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, k_gated_tc<BN>, p) != cudaSuccess) return set_error(cudaGetErrorString(cudaGetLastError()));
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return set_error(cudaGetErrorString(cudaGetLastError()));
   return check_launch();
+}
+
+// ---- products of planes as they are stored --------------------------------------------------
+// The derivative's products: of the weights and the gradients (K runs over units), of the inputs and the gradients (K over cases).
+// One operand's K is its columns, so its tiles arrive with M or N contiguous (boxes of 64 x 64) and tcgen05 reads them so; the
+// scales that lie along K are divided out of the other operand when its planes are written.  Tiles of 256 rows by BN columns a
+// pair of CTAs; the rest as above.
+struct ProductParams {
+  CUtensorMap maps[8];                       // a0 hi, lo, a1 hi, lo, b0 hi, lo, b1 hi, lo
+  int M, N, tiles_m, tiles_n, npairs, nout, k_iters, inv_stride;
+  float* out[2];
+  const float* inv[2];
+  int* status;
+  uint32_t spin_limit, stage_tx;
+};
+
+template <int BN, bool kTrans>
+__global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_constant__ ProductParams p) {
+  using T = Tile<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, bars = base + kRing;
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (kStages + s); };
+  auto done = [&](int a) { return bars + 8u * (2 * kStages + a); };
+  auto free_ = [&](int a) { return bars + 8u * (2 * kStages + 2 + a); };
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  grid_dependents_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t limit = p.spin_limit;
+  const int tiles_n = p.tiles_n * p.nout, tiles = p.tiles_m * tiles_n, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int all_iters = p.k_iters * p.npairs;
+  if (warp == 2 && lane < 8) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.maps[lane]) : "memory");
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kStages; s++) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; a++) {
+      mbar_init(done(a), 1);
+      mbar_init(free_(a), 2 * kEpiThreads / 32);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc2(smem_u32(&tmem_slot), T::kTmemCols);
+    tmem_relinquish2();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  grid_dependency_wait();
+
+  auto gave_up = [&](int code) {
+    if (!*(volatile int*)&abort_flag) atomicCAS(p.status, 0, code);
+    *(volatile int*)&abort_flag = 1;
+  };
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
+    if (warp == 0) {
+      // copies: lanes 0-3 a plane of 64 of this CTA's 128 rows, lanes 4 on a plane of its half of the columns (64 at a time where
+      // they are contiguous)
+      constexpr int kBoxes = kTrans ? BN / 128 : 1;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const bool is_a = lane < 4;
+      const int plane = lane & 1, box = is_a ? lane >> 1 : (lane - 4) >> 1;
+      const uint32_t to = is_a ? plane * 16384u + box * 8192u : 32768u + plane * (uint32_t)(BN * 64) + box * 8192u;
+      for (int t = first; t < tiles && ok; t += step) {
+        int tm, tn;
+        tile_coords_g<8>(t, p.tiles_m, tiles_n, tm, tn);
+        const int o = tn >= p.tiles_n, n0 = (tn - o * p.tiles_n) * BN + (int)rank * (BN / 2);
+        const int row = is_a ? tm * 256 + (int)rank * 128 + 64 * box : n0 + 64 * box;
+        for (int q = 0; q < p.npairs && ok; q++) {
+          const CUtensorMap* map = &p.maps[(is_a ? 2 * q : 4 + 2 * (kTrans ? o : q)) + plane];
+          for (int kb = 0; kb < p.k_iters; kb++) {
+            if (!mbar_wait(empty(stage), phase ^ 1u, &abort_flag, limit)) {
+              gave_up(35);
+              ok = false;
+              break;
+            }
+            const uint32_t bar = full(stage), dst = base + stage * T::kStageBytes + to;
+            if (lane == 0 && rank == 0) mbar_expect_tx(bar, p.stage_tx);
+            if (is_a || (kTrans && lane < 4 + 2 * kBoxes)) tma_load_2d_pair(dst, map, row, kb * kK, bar);
+            else if (!kTrans && lane < 6) tma_load_2d_pair(dst, map, kb * kK, row, bar);
+            if (++stage == T::kNumStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+      }
+      if (!ok)
+        for (int i = 0; i < 1024; i++) __nanosleep(100);
+    } else if (warp == 1 && rank == 0) {
+      const bool elected = elect_one();
+      const uint32_t idesc = (1u << 4) | (1u << 15) | ((kTrans ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((256u >> 4) << 24);
+      // M or N contiguous: blocks of 64 (a row of 128 bytes an element of K) 64 rows apart; sixteen rows a step.  K-major as above.
+      constexpr uint32_t kMn = ((uint32_t)(kK * 128) >> 4) << 16, kStepMn = 2048u >> 4;
+      constexpr uint32_t kB = kTrans ? kMn : 1u << 16, kStepB = kTrans ? kStepMn : 2u;
+      int stage = 0;
+      uint32_t phase = 0, chunk = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        int in_chunk = 0;
+        for (int kb = 0; kb < all_iters; kb++) {
+          const int acc = chunk & 1;
+          if (in_chunk == 0) {
+            if (!mbar_wait(free_(acc), ((chunk >> 1) & 1u) ^ 1u, &abort_flag, limit)) {
+              gave_up(36);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
+          if (!mbar_wait(full(stage), phase, &abort_flag, limit)) {
+            gave_up(37);
+            ok = false;
+            break;
+          }
+          const uint32_t sb = (base + stage * T::kStageBytes) >> 4;
+          const uint32_t a_hi = sb, a_lo = sb + (16384u >> 4), b_hi = sb + (32768u >> 4), b_lo = b_hi + ((uint32_t)(BN * 64) >> 4);
+#pragma unroll
+          for (int i = 0; i < 3; i++) {
+            const uint32_t a = i == 1 ? a_lo : a_hi, b = i == 0 ? b_lo : b_hi;
+#pragma unroll
+            for (int j = 0; j < kK / 16; j++) {
+              const uint64_t da = ((uint64_t)kDescK << 32) | (uint64_t)(kMn + a + kStepMn * j);
+              const uint64_t db = ((uint64_t)kDescK << 32) | (uint64_t)(kB + b + kStepB * j);
+              if (elected) mma_f16_pair(tmem + acc * BN, da, db, idesc, i + j > 0 || in_chunk > 0);
+            }
+          }
+          if (elected) mma_commit_pair(empty(stage), 3);
+          if (++stage == T::kNumStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (++in_chunk == kChunk || kb == all_iters - 1) {
+            if (elected) mma_commit_pair(done(acc), 3);
+            chunk++;
+            in_chunk = 0;
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kDrainRegs));
+    constexpr int kCols = T::kCols, kLoad = kCols < 32 ? kCols : 32;
+    const int ew = warp - 4, q = warp & 3, half = ew >> 2;
+    uint32_t chunk = 0;
+    const int chunks = (all_iters + kChunk - 1) / kChunk;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step) {
+      int tm, tn;
+      tile_coords_g<8>(t, p.tiles_m, tiles_n, tm, tn);
+      const int o = tn >= p.tiles_n, n0 = (tn - o * p.tiles_n) * BN + half * kCols;
+      const int m = tm * 256 + (int)rank * 128 + q * 32 + lane;
+      float sum[kCols];
+#pragma unroll
+      for (int j = 0; j < kCols; j++) sum[j] = 0.0f;
+      for (int c = 0; c < chunks; c++, chunk++) {
+        const int acc = chunk & 1;
+        if (!mbar_wait(done(acc), (chunk >> 1) & 1u, &abort_flag, limit)) {
+          gave_up(38);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * kCols);
+#pragma unroll
+        for (int j = 0; j < kCols; j += kLoad) {
+          float v[kLoad];
+          if constexpr (kLoad == 32) tmem_ld32(from + j, v);
+          else tmem_ld16(from + j, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < kLoad; i++) sum[j + i] += v[i];
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_leader(free_(acc), 0);
+      }
+      if (!ok) break;
+      const float* inv = p.inv[o] + (long)n0 * p.inv_stride;
+      float* out = p.out[o] + (long)n0 * p.M + m;
+      const int live = m < p.M ? p.N - n0 : 0;
+#pragma unroll
+      for (int j = 0; j < kCols; j++)
+        if (j < live) out[(long)j * p.M] = sum[j] * __ldg(inv + (long)j * p.inv_stride);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc2(tmem, T::kTmemCols);
+  }
 }
 
 // ---- matrices as planes --------------------------------------------------------------------
@@ -528,12 +722,56 @@ int gated_tc(const GatedForward& f) {
     if (!plane_map(&p.maps[i], m.p + ((i & 1) ? 0 : lda), (uint64_t)m.rows, (uint64_t)m.cols, 2 * (uint64_t)lda, kK, i < 4 ? 64 : bn / 2))
       return set_error("cuTensorMapEncodeTiled failed for a plane");
   }
+  const long tiles = (long)p.tiles_m * p.tiles_n;
+  if (tiles > 0x7fffffffL) return ERROR_UNSUPPORTED;
+  p.stage_tx = 2 * (32 * 1024 + bn * 128) + (uint32_t)take_injected_bytes();
   switch (bn) {
-    case 256: return launch<256>(p);
-    case 128: return launch<128>(p);
-    case 64: return launch<64>(p);
+    case 256: return launch_pairs(k_gated_tc<256>, p, tiles);
+    case 128: return launch_pairs(k_gated_tc<128>, p, tiles);
+    case 64: return launch_pairs(k_gated_tc<64>, p, tiles);
   }
-  return launch<32>(p);
+  return launch_pairs(k_gated_tc<32>, p, tiles);
+}
+
+int plane_product(const PlaneProduct& f) {
+  ProductParams p = {};
+  p.M = f.a[0].rows;
+  p.N = f.trans ? f.b[0].rows : f.b[0].cols;
+  p.npairs = f.npairs;
+  p.nout = f.nout;
+  p.k_iters = (f.a[0].cols + kK - 1) / kK;
+  p.inv_stride = f.inv_stride;
+  for (int i = 0; i < f.nout; i++) {
+    p.out[i] = f.out[i];
+    p.inv[i] = f.inv[i];
+  }
+  p.status = status_word();
+  p.spin_limit = wait_limit();
+  p.tiles_m = (p.M + 255) / 256;
+  // the wider tile reads less shared memory a multiply-add; the narrower one where it needs fewer turns of the pairs
+  const long pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
+  auto turns = [&](int w) { return ((long)p.tiles_m * f.nout * ((p.N + w - 1) / w) + pairs - 1) / pairs; };
+  const int bn = 2 * turns(256) <= turns(128) * 1.1 ? 256 : 128;
+  p.tiles_n = (p.N + bn - 1) / bn;
+  const long tiles = (long)p.tiles_m * p.tiles_n * f.nout;
+  if (tiles > 0x7fffffffL) return ERROR_UNSUPPORTED;
+  const int nb = f.trans ? f.nout : f.npairs;
+  for (int i = 0; i < 8; i++) {
+    const int which = (i >> 1) & 1;
+    const bool is_a = i < 4;
+    if (which >= (is_a ? f.npairs : nb)) {
+      p.maps[i] = p.maps[i - 2];
+      continue;
+    }
+    const Planes& m = is_a ? f.a[which] : f.b[which];
+    const int lda = aux_rows(m.rows);
+    if (!plane_map(&p.maps[i], m.p + ((i & 1) ? 0 : lda), (uint64_t)m.rows, (uint64_t)m.cols, 2 * (uint64_t)lda, kK,
+                   is_a || f.trans ? kK : bn / 2))
+      return set_error("cuTensorMapEncodeTiled failed for a plane");
+  }
+  p.stage_tx = 2 * (32 * 1024 + bn * 128) + (uint32_t)take_injected_bytes();
+  if (f.trans) return bn == 256 ? launch_pairs(k_plane_product<256, true>, p, tiles) : launch_pairs(k_plane_product<128, true>, p, tiles);
+  return bn == 256 ? launch_pairs(k_plane_product<256, false>, p, tiles) : launch_pairs(k_plane_product<128, false>, p, tiles);
 }
 
 }  // namespace b200

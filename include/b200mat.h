@@ -311,9 +311,10 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
  * tensor cores run; they have to be filled again when the weights change. */
 int gated_planes(cudamat* gate_w, cudamat* up_w, cudamat* gate_planes, cudamat* up_planes, cudamat* scales);
 /* deriv: the gradient of gated_product's target.  gate and up, as it left them, are overwritten with their gradients; the others
- * receive those of mat, weights and biases (null: not wanted), summed in a fixed order. */
+ * receive those of mat, weights and biases (null: not wanted), summed in a fixed order.  Planes as in gated_product. */
 int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gate_w, cudamat* up_w, cudamat* mat, int activation,
-                        cudamat* grad_mat, cudamat* grad_gate_w, cudamat* grad_up_w, cudamat* grad_gate_bias, cudamat* grad_up_bias);
+                        cudamat* gate_planes, cudamat* up_planes, cudamat* scales, cudamat* grad_mat, cudamat* grad_gate_w,
+                        cudamat* grad_up_w, cudamat* grad_gate_bias, cudamat* grad_up_bias);
 
 /* target = add + (u > dropprob ? mat / (1 - dropprob) : 0), add (or null: 0) of mat's shape, u the uniforms that fill_with_rand would
  * draw.  Consumes one sampling call.  No mask is stored: the same seed and call number draw it again (on the gradient: without add).

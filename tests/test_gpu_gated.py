@@ -302,3 +302,81 @@ def test_two_recorded_forward_passes_share_no_scratch(cm):
     for s, w in zip(sets, want):
         assert np.array_equal(get(s[3]), w)
     assert cm.read_status() == 0
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("shape", SHAPES + [(64, 128, 256), (65, 129, 257), (40, 600, 33), (700, 300, 70), (130, 1000, 600), (257, 9, 1300), (520, 513, 127)])
+def test_derivative_on_tensor_cores_and_cuda_cores(cm, shape, path):
+    """Gradients of units, cases and weights whose magnitudes lie far apart: none costs another its bits."""
+    V, H, N = shape
+    rng = np.random.default_rng(V * 5 + H * 3 + N)
+    wg, wu = (np.ldexp(rng.standard_normal((V, H)), rng.integers(-20, 5, (1, H))).astype(np.float32) for _ in range(2))
+    x = np.ldexp(rng.standard_normal((V, N)), rng.integers(-20, 5, (1, N))).astype(np.float32)
+    gate, up = (rng.standard_normal((H, N)).astype(np.float32) for _ in range(2))
+    dy = np.ldexp(rng.standard_normal((H, N)), rng.integers(-25, 5, (H, 1)) + rng.integers(-25, 5, (1, N))).astype(np.float32)
+    dy[:, N // 2] = 0                          # a case without weight
+    G = cm.CUDAMatrix
+    ga, gb, gx = G(wg), G(wu), G(x)
+    dx, dwg, dwu, dbg, dbu = cm.empty((V, N)), cm.empty((V, H)), cm.empty((V, H)), cm.empty((H, 1)), cm.empty((1, H))
+    gm, um = G(gate), G(up)
+    out = dict(grad_x=dx, grad_gate_w=dwg, grad_up_w=dwu, grad_gate_bias=dbg, grad_up_bias=dbu)
+    on_path(cm, path, lambda: cm.gated_product_deriv(G(dy), gm, um, ga, gb, gx, activation="relu", **out))
+    dg, du = dy * up * (gate > 0), dy * np.maximum(gate, 0)      # one rounding a product
+    assert np.array_equal(get(gm), dg) and np.array_equal(get(um), du)
+    A, B, X, D, E = (v.astype(np.float64) for v in (wg, wu, x, dg, du))
+    of_case = np.maximum((np.abs(A).max(0)[:, None] * np.abs(D)).max(0), (np.abs(B).max(0)[:, None] * np.abs(E)).max(0))
+    size = np.abs(A) @ np.abs(D) + np.abs(B) @ np.abs(E)
+    within(get(dx), A @ D + B @ E, ((2 * H + 4) * U + 2.0 ** -18) * size + 2.0 ** -30 * 2 * H * of_case[None] + 1e-37)
+    assert (get(dx)[:, N // 2] == 0).all()
+    for got, d in ((dwg, D), (dwu, E)):
+        of_unit = (np.abs(d) * np.abs(X).max(0)[None]).max(1)
+        within(get(got), X @ d.T, ((N + 4) * U + 2.0 ** -18) * (np.abs(X) @ np.abs(d).T) + 2.0 ** -30 * N * of_unit[None] + 1e-37)
+    within(get(dbg)[:, 0], D.sum(1), (N + 8) * U * np.abs(D).sum(1) + 1e-37)
+    within(get(dbu)[0], E.sum(1), (N + 8) * U * np.abs(E).sum(1) + 1e-37)
+    want = {k: get(v) for k, v in out.items()}
+    # each gradient alone, and with the weights' planes: the same bits
+    planes = cm.GatedPlanes(ga, gb)
+    for names in (["grad_x"], ["grad_gate_w"], ["grad_up_w", "grad_x"], ["grad_up_bias"], []):
+        for name in names:
+            out[name].assign(3.0)
+        on_path(cm, path, lambda: cm.gated_product_deriv(G(dy), G(gate), G(up), ga, gb, gx, activation="relu", planes=planes,
+                                                         **{k: out[k] for k in names}))
+        for name in names:
+            assert np.array_equal(get(out[name]), want[name]), name
+    assert cm.read_status() == 0
+
+
+def test_two_recorded_derivatives_share_no_scratch(cm):
+    rng = np.random.default_rng(18)
+    torch.zeros(1, device="cuda")
+    sets, streams, graphs = [], [], [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    for V, H, N in ((700, 900, 300), (1300, 500, 200)):
+        r = lambda *s: cm.CUDAMatrix(rng.standard_normal(s).astype(np.float32))
+        s = dict(w=(r(V, H), r(V, H)), x=r(V, N), dy=r(H, N), gate=r(H, N), up=r(H, N), g=cm.empty((H, N)), u=cm.empty((H, N)),
+                 out=dict(grad_x=cm.empty((V, N)), grad_gate_w=cm.empty((V, H)), grad_up_w=cm.empty((V, H)), grad_up_bias=cm.empty((H, 1))))
+        sets.append(s)
+
+    def step(s):
+        s["g"].assign(s["gate"])
+        s["u"].assign(s["up"])
+        cm.gated_product_deriv(s["dy"], s["g"], s["u"], *s["w"], s["x"], activation="gelu", **s["out"])
+    for s, graph in zip(sets, graphs):
+        with _On(cm, graph) as on:
+            on_path(cm, 1, lambda: step(s))
+        streams.append(on.stream)
+    want = []
+    for s in sets:
+        on_path(cm, 1, lambda: step(s))
+        want.append({k: get(v) for k, v in s["out"].items()})
+        for v in s["out"].values():
+            v.assign(0)
+    cm.cuda_sync_threads()
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for s, w in zip(sets, want):
+        for k, v in s["out"].items():
+            assert np.array_equal(get(v), w[k]), k
+    assert cm.read_status() == 0

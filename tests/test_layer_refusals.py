@@ -130,7 +130,8 @@ def test_gated_product_refuses():
 def test_gated_product_deriv_refuses():
     def f(dy=None, gate=None, up=None, wg=None, wu=None, x=None, act=1, out=(None,) * 5):
         d = lambda m, r, c: m if m is not None else mat(r, c)
-        return cm._lib.gated_product_deriv(d(dy, 7, 5), d(gate, 7, 5), d(up, 7, 5), d(wg, 9, 7), d(wu, 9, 7), d(x, 9, 5), ct.c_int(act), *out)
+        return cm._lib.gated_product_deriv(d(dy, 7, 5), d(gate, 7, 5), d(up, 7, 5), d(wg, 9, 7), d(wu, 9, 7), d(x, 9, 5), ct.c_int(act),
+                                          None, None, None, *out)
     assert f(dy=mat(7, 4)) == DIMENSIONS and f(up=mat(5, 7)) == DIMENSIONS and f(wu=mat(7, 9)) == DIMENSIONS
     assert f(out=(mat(9, 4), None, None, None, None)) == DIMENSIONS
     assert f(out=(None, mat(7, 9), None, None, None)) == DIMENSIONS
