@@ -19,6 +19,20 @@ struct GatedArgs {
   int V, H, N;
 };
 
+template <int kVec>
+__device__ __forceinline__ void load(const float* p, float (&v)[kVec]) {
+  if constexpr (kVec == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  } else {
+    v[0] = *p;
+  }
+}
+template <int kVec>
+__device__ __forceinline__ void store(float* p, const float (&v)[kVec]) {
+  if constexpr (kVec == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else *p = v[0];
+}
 // 64 units by 64 cases a block of 256 threads, four by four of both products a thread, full fp32 multiply-adds.
 template <int kAct>
 __global__ void __launch_bounds__(256) k_gated_simt(const GatedArgs a) {
@@ -65,25 +79,100 @@ __global__ void __launch_bounds__(256) k_gated_simt(const GatedArgs a) {
     }
 }
 
+// Up to kN cases: every weight is read once, by a warp a unit (kWarps 1) or a block's eight, which both products of a unit share;
+// the cases come from L1.  Full fp32 multiply-adds.  Bound by HBM: 8 bytes a weight pair.
+constexpr int kFewCases = 8;
+template <int kN, int kVec, int kWarps>
+__global__ void __launch_bounds__(256) k_gated_few(const GatedArgs a, int activation) {
+  __shared__ float red[kWarps > 1 ? kWarps : 1][2 * kN];
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const long u = kWarps > 1 ? (long)blockIdx.x : (long)blockIdx.x * 8 + wid;
+  if (u >= a.H) return;
+  constexpr int kBatch = kVec == 4 ? 4 : 8;
+  const float *wg = a.wg + u * a.V, *wu = a.wu + u * a.V;
+  float sum[2 * kN];
+#pragma unroll
+  for (int i = 0; i < 2 * kN; i++) sum[i] = 0.0f;
+  const int step = 32 * kWarps, items = a.V / kVec;
+  for (int base = (kWarps > 1 ? wid * 32 : 0) + lane; base < items; base += kBatch * step) {
+    float g[kBatch][kVec], w[kBatch][kVec];
+#pragma unroll
+    for (int b = 0; b < kBatch; b++) {
+      const int i = base + b * step;
+      if (i < items) {
+        load<kVec>(wg + (long)i * kVec, g[b]);
+        load<kVec>(wu + (long)i * kVec, w[b]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; j++) g[b][j] = w[b][j] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; b++) {
+      const int i = base + b * step;
+      if (i >= items) continue;
+#pragma unroll
+      for (int n = 0; n < kN; n++) {
+        if (n >= a.N) continue;
+        float x[kVec];
+        load<kVec>(a.x + (long)n * a.V + (long)i * kVec, x);
+#pragma unroll
+        for (int j = 0; j < kVec; j++) {
+          sum[2 * n] = fmaf(g[b][j], x[j], sum[2 * n]);
+          sum[2 * n + 1] = fmaf(w[b][j], x[j], sum[2 * n + 1]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * kN; i++)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+  if (kWarps > 1) {
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < 2 * kN; i++) red[wid][i] = sum[i];
+    __syncthreads();
+    if (wid) return;
+#pragma unroll
+    for (int i = 0; i < 2 * kN; i++) {
+      sum[i] = red[0][i];
+#pragma unroll
+      for (int k = 1; k < kWarps; k++) sum[i] += red[k][i];
+    }
+  }
+  float gv = 0.0f, uv = 0.0f;      // lane n finishes case n
+#pragma unroll
+  for (int n = 0; n < kN; n++)
+    if (lane == n) {
+      gv = sum[2 * n];
+      uv = sum[2 * n + 1];
+    }
+  if (lane >= kN || lane >= a.N) return;
+  if (a.bg) gv += a.bg[u];
+  if (a.bu) uv += a.bu[u];
+  const long at = (long)lane * a.H + u;
+  if (a.gate) {
+    a.gate[at] = gv;
+    a.up[at] = uv;
+  }
+  float slope;
+  switch (activation) {
+    case kLogistic: gv = activate<kLogistic>(gv, slope); break;
+    case kRelu: gv = activate<kRelu>(gv, slope); break;
+    case kSilu: gv = activate<kSilu>(gv, slope); break;
+    case kGelu: gv = activate<kGelu>(gv, slope); break;
+  }
+  a.y[at] = gv * uv;
+}
+
 // ---- the derivative's elementwise part ------------------------------------------------------
 // A thread takes kVec units of some cases, one case after another: the units' sums and maxima stay in registers.  Bound by HBM:
 // 20 bytes a unit and case for the gradients, 8 + 16 for their planes.
 constexpr int kMostCases = 64, kDerivThreads = 128;
 
-template <int kVec>
-__device__ __forceinline__ void load(const float* p, float (&v)[kVec]) {
-  if constexpr (kVec == 4) {
-    const float4 x = *reinterpret_cast<const float4*>(p);
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-  } else {
-    v[0] = *p;
-  }
-}
-template <int kVec>
-__device__ __forceinline__ void store(float* p, const float (&v)[kVec]) {
-  if constexpr (kVec == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  else *p = v[0];
-}
 __device__ __forceinline__ uint32_t magnitude(float v) {      // bits of finite magnitudes, in their order
   const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0u;
@@ -243,8 +332,7 @@ int bias_ok(const cudamat* v, int h) {
   return numel(v) == h && (v->size[0] == 1 || v->size[1] == 1) ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
 }
 bool is(const cudamat* m, int rows, int cols) { return m->size[0] == rows && m->size[1] == cols; }
-constexpr long kTensorDerivWork = 1L << 40;
-constexpr long kTensorWork = 1L << 21;      // multiply-adds of one of the products from which the tensor cores take both
+constexpr long kTensorWork = 1L << 18;      // multiply-adds of one of the products from which the tensor cores take both
 int weights_ok(const cudamat* gate_w, const cudamat* up_w) {
   if (!gate_w->on_device || !up_w->on_device) return ERROR_NOT_ON_DEVICE;
   if (gate_w->is_trans || up_w->is_trans) return ERROR_TRANSPOSED;
@@ -329,6 +417,25 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
   }
   if (H == 0 || N == 0) return 0;
   auto at = [](cudamat* m) { return m ? m->data_device : nullptr; };
+  if (N <= kFewCases && gemm_path() == 0) {
+    const GatedArgs a = {gate_w->data_device, up_w->data_device, mat->data_device, at(gate_bias), at(up_bias),
+                         at(gate),            at(up),            target->data_device, V, H, N};
+    const bool vec = V % 4 == 0 && on16(a.wg) && on16(a.wu) && on16(a.x), block = H < 16L * sm_count() && V >= 512;
+    const dim3 grid(block ? H : (H + 7) / 8);
+#define FEW(CASES)                                                                                                                \
+  do {                                                                                                                            \
+    if (vec && block) (void)launch_dependent(k_gated_few<CASES, 4, 8>, grid, dim3(256), 0, stream(), a, activation);               \
+    else if (vec) (void)launch_dependent(k_gated_few<CASES, 4, 1>, grid, dim3(256), 0, stream(), a, activation);                   \
+    else if (block) (void)launch_dependent(k_gated_few<CASES, 1, 8>, grid, dim3(256), 0, stream(), a, activation);                 \
+    else (void)launch_dependent(k_gated_few<CASES, 1, 1>, grid, dim3(256), 0, stream(), a, activation);                            \
+  } while (0)
+    if (N == 1) FEW(1);
+    else if (N == 2) FEW(2);
+    else if (N <= 4) FEW(4);
+    else FEW(8);
+#undef FEW
+    return check_launch();
+  }
   // Tensor cores, behind a launch or two that split the operands: where the products are more than those cost.
   const bool large = (long)V * H * N >= kTensorWork;
   if (V > 0 && gemm_path() != 2 && (large || gemm_path() == 1) && tma_available()) {
@@ -394,7 +501,14 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     return 0;
   }
   const bool biases = grad_gate_bias || grad_up_bias, weights = grad_gate_w || grad_up_w;
-  const bool large = (long)V * H * N >= kTensorDerivWork;
+  // On planes, or as four products of the matrices themselves (`dot`), which read large weights faster for few cases and spend less
+  // on tiny layers, but take matrices that TMA cannot address behind copies.  Microseconds, planes / dot: 256 x 256, 32 cases 33 / 28;
+  // 784 x 500, 100 cases 41 / 40; 1024 x 1024, 128 cases 42 / 52; 2048 x 8192, 64 cases 190 / 149, 256 cases 228 / 233, 4096 cases
+  // 1402 / 2462; 301 x 301, 301 cases 43 / 61; 1357 x 601, 203 cases 42 / 103.
+  const bool aligned = V % 4 == 0 && H % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device) &&
+                       on16(gate->data_device) && on16(up->data_device);
+  const bool few = aligned && !gate_planes && N < 256 && (long)V * H >= 1L << 22;
+  const bool large = (long)V * H * N >= 1L << (aligned ? 26 : 22) && !few;
   const bool tc = V > 0 && (weights || grad_mat) && gemm_path() != 2 && (large || gemm_path() == 1) && tma_available();
   const int cases = gated_deriv_cases(H, N), blocks = (N + cases - 1) / cases;
   const bool split_w = tc && !gate_planes;
@@ -434,9 +548,7 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     const SplitJob jobs[3] = {{mat->data_device, (uint16_t*)xp.p, (float*)d.x_inv, 1, N},
                               {gate_w->data_device, (uint16_t*)wgp.p, (float*)d.w_inv, 2, H},
                               {up_w->data_device, (uint16_t*)wup.p, (float*)d.w_inv + 1, 2, H}};
-    if (cudaMemsetAsync(p + at_tmax, 0, after_max - at_tmax, stream()) != cudaSuccess)
-      return set_error(cudaGetErrorString(cudaGetLastError()));
-    if ((err = split_columns(jobs, split_w ? 3 : 1, V))) return err;
+    if ((err = split_columns(jobs, split_w ? 3 : 1, V, d.token_max, (int)((after_max - at_tmax) / 4)))) return err;
   }
   if ((err = gated_deriv(d))) return err;
   if (biases) {

@@ -42,8 +42,8 @@ struct SplitJob {
   float* inv;
   int inv_stride, cols;
 };
-// Up to three matrices of the same number of rows, in one launch.
-int split_columns(const SplitJob* jobs, int njobs, int rows);
+// Up to three matrices of the same number of rows, in one launch, which sets nzero words to zero too.
+int split_columns(const SplitJob* jobs, int njobs, int rows, uint32_t* zero = nullptr, int nzero = 0);
 
 // y = act(Wg' x + bg) * (Wu' x + bu); w_inv: 2 x H, gate's and up's
 struct GatedForward {

@@ -356,11 +356,28 @@ int launch_pairs(void (*kernel)(Params), const Params& p, long tiles) {
 struct ProductParams {
   CUtensorMap maps[8];                       // a0 hi, lo, a1 hi, lo, b0 hi, lo, b1 hi, lo
   int M, N, tiles_m, tiles_n, npairs, nout, k_iters, inv_stride;
+  int splits;                                // > 1: each tile's stages are shared out; split s leaves its sums in part + s * M * N
+  float* part;
   float* out[2];
   const float* inv[2];
   int* status;
   uint32_t spin_limit, stage_tx;
 };
+
+// The splits' sums in order, times the columns' scales.
+__global__ void __launch_bounds__(256) k_plane_finish(const __grid_constant__ ProductParams p) {
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const long n = (long)p.M * p.N, all = n * p.nout;
+  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long)gridDim.x * blockDim.x) {
+    float s = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < p.splits; k++) s += p.part[all * k + i];
+    const int o = i >= n;
+    const long at = i - o * n;
+    p.out[o][at] = s * p.inv[o][at / p.M * p.inv_stride];
+  }
+}
 
 template <int BN, bool kTrans>
 __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_constant__ ProductParams p) {
@@ -377,8 +394,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const uint32_t limit = p.spin_limit;
-  const int tiles_n = p.tiles_n * p.nout, tiles = p.tiles_m * tiles_n, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int tiles_n = p.tiles_n * p.nout, splits = p.splits, items = p.tiles_m * tiles_n * splits, first = blockIdx.x >> 1, step = gridDim.x >> 1;
   const int all_iters = p.k_iters * p.npairs;
+  auto of_split = [&](int s) { return (int)((long)all_iters * s / splits); };     // its first stage
   if (warp == 2 && lane < 8) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.maps[lane]) : "memory");
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -420,27 +438,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
       const bool is_a = lane < 4;
       const int plane = lane & 1, box = is_a ? lane >> 1 : (lane - 4) >> 1;
       const uint32_t to = is_a ? plane * 16384u + box * 8192u : 32768u + plane * (uint32_t)(BN * 64) + box * 8192u;
-      for (int t = first; t < tiles && ok; t += step) {
+      for (int w = first; w < items && ok; w += step) {
         int tm, tn;
-        tile_coords_g<8>(t, p.tiles_m, tiles_n, tm, tn);
+        tile_coords_g<8>(w / splits, p.tiles_m, tiles_n, tm, tn);
         const int o = tn >= p.tiles_n, n0 = (tn - o * p.tiles_n) * BN + (int)rank * (BN / 2);
         const int row = is_a ? tm * 256 + (int)rank * 128 + 64 * box : n0 + 64 * box;
-        for (int q = 0; q < p.npairs && ok; q++) {
+        const int last = of_split(w % splits + 1);
+        int it = of_split(w % splits), q = it / p.k_iters, kb = it - q * p.k_iters;
+        for (; it < last; it++) {
           const CUtensorMap* map = &p.maps[(is_a ? 2 * q : 4 + 2 * (kTrans ? o : q)) + plane];
-          for (int kb = 0; kb < p.k_iters; kb++) {
-            if (!mbar_wait(empty(stage), phase ^ 1u, &abort_flag, limit)) {
-              gave_up(35);
-              ok = false;
-              break;
-            }
-            const uint32_t bar = full(stage), dst = base + stage * T::kStageBytes + to;
-            if (lane == 0 && rank == 0) mbar_expect_tx(bar, p.stage_tx);
-            if (is_a || (kTrans && lane < 4 + 2 * kBoxes)) tma_load_2d_pair(dst, map, row, kb * kK, bar);
-            else if (!kTrans && lane < 6) tma_load_2d_pair(dst, map, kb * kK, row, bar);
-            if (++stage == T::kNumStages) {
-              stage = 0;
-              phase ^= 1u;
-            }
+          if (!mbar_wait(empty(stage), phase ^ 1u, &abort_flag, limit)) {
+            gave_up(35);
+            ok = false;
+            break;
+          }
+          const uint32_t bar = full(stage), dst = base + stage * T::kStageBytes + to;
+          if (lane == 0 && rank == 0) mbar_expect_tx(bar, p.stage_tx);
+          if (is_a || (kTrans && lane < 4 + 2 * kBoxes)) tma_load_2d_pair(dst, map, row, kb * kK, bar);
+          else if (!kTrans && lane < 6) tma_load_2d_pair(dst, map, kb * kK, row, bar);
+          if (++stage == T::kNumStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (++kb == p.k_iters) {
+            kb = 0;
+            q++;
           }
         }
       }
@@ -455,9 +477,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
       int stage = 0;
       uint32_t phase = 0, chunk = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
+      for (int w = first; w < items && ok; w += step) {
         int in_chunk = 0;
-        for (int kb = 0; kb < all_iters; kb++) {
+        const int iters = of_split(w % splits + 1) - of_split(w % splits);
+        for (int kb = 0; kb < iters; kb++) {
           const int acc = chunk & 1;
           if (in_chunk == 0) {
             if (!mbar_wait(free_(acc), ((chunk >> 1) & 1u) ^ 1u, &abort_flag, limit)) {
@@ -489,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
             stage = 0;
             phase ^= 1u;
           }
-          if (++in_chunk == kChunk || kb == all_iters - 1) {
+          if (++in_chunk == kChunk || kb == iters - 1) {
             if (elected) mma_commit_pair(done(acc), 3);
             chunk++;
             in_chunk = 0;
@@ -502,13 +525,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
     constexpr int kCols = T::kCols, kLoad = kCols < 32 ? kCols : 32;
     const int ew = warp - 4, q = warp & 3, half = ew >> 2;
     uint32_t chunk = 0;
-    const int chunks = (all_iters + kChunk - 1) / kChunk;
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += step) {
+    for (int w = first; w < items && ok; w += step) {
       int tm, tn;
-      tile_coords_g<8>(t, p.tiles_m, tiles_n, tm, tn);
+      tile_coords_g<8>(w / splits, p.tiles_m, tiles_n, tm, tn);
       const int o = tn >= p.tiles_n, n0 = (tn - o * p.tiles_n) * BN + half * kCols;
       const int m = tm * 256 + (int)rank * 128 + q * 32 + lane;
+      const int sp = w % splits, chunks = (of_split(sp + 1) - of_split(sp) + kChunk - 1) / kChunk;
       float sum[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; j++) sum[j] = 0.0f;
@@ -535,9 +558,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
         if (lane == 0) mbar_arrive_leader(free_(acc), 0);
       }
       if (!ok) break;
+      const int live = m < p.M ? p.N - n0 : 0;
+      if (splits > 1) {
+        float* part = p.part + ((long)sp * p.nout + o) * p.M * p.N + (long)n0 * p.M + m;
+#pragma unroll
+        for (int j = 0; j < kCols; j++)
+          if (j < live) part[(long)j * p.M] = sum[j];
+        continue;
+      }
       const float* inv = p.inv[o] + (long)n0 * p.inv_stride;
       float* out = p.out[o] + (long)n0 * p.M + m;
-      const int live = m < p.M ? p.N - n0 : 0;
 #pragma unroll
       for (int j = 0; j < kCols; j++)
         if (j < live) out[(long)j * p.M] = sum[j] * __ldg(inv + (long)j * p.inv_stride);
@@ -557,6 +587,8 @@ struct SplitJobs {
   SplitJob job[3];
   int first[3];          // each one's first block: of eight columns, or of one
   int h, lda;
+  uint32_t* zero;        // words that later launches count in
+  int nzero;
 };
 
 // A column's exponent from its largest finite magnitude (m: its bits), and its inverse scale written.
@@ -589,6 +621,7 @@ __global__ void __launch_bounds__(256) k_split_columns(const __grid_constant__ S
   __shared__ uint32_t red[8];
   grid_dependents_launch();
   grid_dependency_wait();
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < a.nzero; i += gridDim.x * 256) a.zero[i] = 0;
   const int which = blockIdx.x >= a.first[2] ? 2 : blockIdx.x >= a.first[1] ? 1 : 0;
   const float* src = which == 2 ? a.job[2].x : which ? a.job[1].x : a.job[0].x;
   uint16_t* planes = which == 2 ? a.job[2].planes : which ? a.job[1].planes : a.job[0].planes;
@@ -651,8 +684,10 @@ __global__ void __launch_bounds__(256) k_split_columns(const __grid_constant__ S
 
 }  // namespace
 
-int split_columns(const SplitJob* jobs, int njobs, int rows) {
+int split_columns(const SplitJob* jobs, int njobs, int rows, uint32_t* zero, int nzero) {
   SplitJobs a = {};
+  a.zero = zero;
+  a.nzero = nzero;
   a.h = rows;
   a.lda = aux_rows(rows);
   bool vec = rows % 4 == 0;
@@ -753,7 +788,15 @@ int plane_product(const PlaneProduct& f) {
   auto turns = [&](int w) { return ((long)p.tiles_m * f.nout * ((p.N + w - 1) / w) + pairs - 1) / pairs; };
   const int bn = 2 * turns(256) <= turns(128) * 1.1 ? 256 : 128;
   p.tiles_n = (p.N + bn - 1) / bn;
-  const long tiles = (long)p.tiles_m * p.tiles_n * f.nout;
+  // too few tiles for the device and long sums: each tile's stages are shared out, eight or more to a pair
+  const int all_iters = p.k_iters * f.npairs;
+  long splits = pairs / ((long)p.tiles_m * p.tiles_n * f.nout);
+  if (splits > all_iters / 8) splits = all_iters / 8;
+  p.splits = splits < 1 ? 1 : (int)splits;
+  CallScratch room(2, p.splits > 1 ? (size_t)p.splits * f.nout * p.M * p.N * sizeof(float) : 0);
+  p.part = (float*)room.p;
+  if (p.splits > 1 && !p.part) return CUDA_ERROR;
+  const long tiles = (long)p.tiles_m * p.tiles_n * f.nout * p.splits;
   if (tiles > 0x7fffffffL) return ERROR_UNSUPPORTED;
   const int nb = f.trans ? f.nout : f.npairs;
   for (int i = 0; i < 8; i++) {
@@ -770,8 +813,14 @@ int plane_product(const PlaneProduct& f) {
       return set_error("cuTensorMapEncodeTiled failed for a plane");
   }
   p.stage_tx = 2 * (32 * 1024 + bn * 128) + (uint32_t)take_injected_bytes();
-  if (f.trans) return bn == 256 ? launch_pairs(k_plane_product<256, true>, p, tiles) : launch_pairs(k_plane_product<128, true>, p, tiles);
-  return bn == 256 ? launch_pairs(k_plane_product<256, false>, p, tiles) : launch_pairs(k_plane_product<128, false>, p, tiles);
+  int err;
+  if (f.trans) err = bn == 256 ? launch_pairs(k_plane_product<256, true>, p, tiles) : launch_pairs(k_plane_product<128, true>, p, tiles);
+  else err = bn == 256 ? launch_pairs(k_plane_product<256, false>, p, tiles) : launch_pairs(k_plane_product<128, false>, p, tiles);
+  if (err || p.splits == 1) return err;
+  long blocks = ((long)p.M * p.N * f.nout + 255) / 256;
+  if (blocks > 8L * sm_count()) blocks = 8L * sm_count();
+  (void)launch_dependent(k_plane_finish, dim3((unsigned)blocks), dim3(256), 0, stream(), p);
+  return check_launch();
 }
 
 }  // namespace b200
