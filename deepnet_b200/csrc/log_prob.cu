@@ -3,9 +3,10 @@
 //   log p_t = d_t - log s,   H = log s - (sum exp(d) d) / s
 //   dz_i = g (1[i = t] - p_i) - q p_i (log p_i + H)      for gradients g of log p_t and q of H
 // The logits are read once: every thread carries m, s and sum exp(d) d of what it has seen, joined by warps, then by the
-// block.  Bound by HBM (4 bytes a logit forward, 8 back).  The k likeliest are kept sorted across a warp's lanes (k <= 32) by
-// (value, lower index first); a value that beats the warp's k-th is put in its place with two shuffles, which for logits in
-// no order happens k (1 + ln(n / k)) times in n; the warps' lists are joined at the end.
+// block.  Bound by HBM (4 bytes a logit forward, 8 back).  For the k likeliest (k <= 32, equal logits by the lower number) the
+// threads' maxima give a bound that at least k logits reach and few others do: the column is read again, from L1 or L2, and
+// what reaches the bound is ranked (50 021 words of normal logits, k 20: about 60).  Where more than 512 do, or a mask leaves
+// fewer than k, sorted lists across the lanes of each warp find them, slowly where many logits rise above all before them.
 // A column whose logits are all -inf has no distribution: log p is -inf, H 0 and the gradient 0.  A NaN or +inf among a
 // column's logits makes all its results NaN (its likeliest tokens are then 0, 1, ...).
 #include "common.cuh"
@@ -95,89 +96,106 @@ __device__ __forceinline__ void store(float* p, long i, const float (&v)[kVec]) 
   else p[i] = v[0];
 }
 
+// A float's bits in the floats' order, and back (0: below all).
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+constexpr int kCandidates = 512;
+
 // kBatch groups of kVec logits of a thread, all read before the first is used.
 template <int kVec, bool kTop>
 __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a) {
   constexpr int kBatch = kVec == 4 ? 2 : 8;
   __shared__ Sums sums[32];
-  __shared__ Top lists[32 * kMostTop];
+  __shared__ uint32_t bounds[32];
+  __shared__ Top lists[kTop ? 32 * kMostTop : 1], candidates[kTop ? kCandidates : 1];
+  __shared__ int count;
   grid_dependents_launch();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const long c = blockIdx.x;
   const float* col = a.z + c * a.h;
   Sums s = {-INFINITY, 0.0f, 0.0f};
-  Top top = {-INFINITY, 0x7fffffff};
-  float kv = -INFINITY;
-  int ki = 0x7fffffff;
   const int items = a.h / kVec;                        // (kVec 4: h is a multiple)
-  for (int base = 0; base < items; base += kBatch * (int)blockDim.x) {
-    float v[kBatch][kVec];
+  // f(value, its number) for every logit of this thread (-inf, 0x7fffffff beyond the last); all threads of a block go round together
+  auto each = [&](auto before, auto f) {
+    for (int base = 0; base < items; base += kBatch * (int)blockDim.x) {
+      float v[kBatch][kVec];
 #pragma unroll
-    for (int b = 0; b < kBatch; b++) {
-      const int i = base + b * (int)blockDim.x + (int)threadIdx.x;
-      if (i < items) {
-        load<kVec>(col, i, v[b]);
-      } else {
+      for (int b = 0; b < kBatch; b++) {
+        const int i = base + b * (int)blockDim.x + (int)threadIdx.x;
+        if (i < items) {
+          load<kVec>(col, i, v[b]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kVec; j++) v[b][j] = -INFINITY;
+          for (int j = 0; j < kVec; j++) v[b][j] = -INFINITY;
+        }
       }
-    }
-    float m = s.m;
-#pragma unroll
-    for (int b = 0; b < kBatch; b++)
-#pragma unroll
-      for (int j = 0; j < kVec; j++) m = fmaxf(m, v[b][j]);
-    if (m > s.m) {
-      const float d = s.m - m, f = expf(d);
-      s.t = f > 0.0f ? (s.t + d * s.s) * f : 0.0f * s.s;
-      s.s *= f;
-      s.m = m;
-    }
-#pragma unroll
-    for (int b = 0; b < kBatch; b++)
-#pragma unroll
-      for (int j = 0; j < kVec; j++) {
-        // (a maximum of -inf: nothing to add but a NaN)
-        const float d = v[b][j] == -INFINITY ? -INFINITY : v[b][j] - m, e = expf(d);
-        s.s += e;
-        s.t += e > 0.0f ? e * d : e;
-      }
-    if (kTop) {
+      before(v);
 #pragma unroll
       for (int b = 0; b < kBatch; b++)
 #pragma unroll
         for (int j = 0; j < kVec; j++) {
           const int i = base + b * (int)blockDim.x + (int)threadIdx.x;
-          offer(top, a.k, v[b][j], i < items ? kVec * i + j : 0x7fffffff, kv, ki);
+          f(v[b][j], i < items ? kVec * i + j : 0x7fffffff);
         }
     }
-  }
+  };
+  each(
+      [&](float (&v)[kBatch][kVec]) {
+        float m = s.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums x;
-    x.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-    x.s = __shfl_xor_sync(0xffffffffu, s.s, o);
-    x.t = __shfl_xor_sync(0xffffffffu, s.t, o);
-    s = (threadIdx.x & o) ? join(x, s) : join(s, x);         // (the same order in both lanes: the same bits)
+        for (int b = 0; b < kBatch; b++)
+#pragma unroll
+          for (int j = 0; j < kVec; j++) m = fmaxf(m, v[b][j]);
+        if (m > s.m) {
+          const float d = s.m - m, f = expf(d);
+          s.t = f > 0.0f ? (s.t + d * s.s) * f : 0.0f * s.s;
+          s.s *= f;
+          s.m = m;
+        }
+      },
+      [&](float v, int) {
+        // (a maximum of -inf: nothing to add but a NaN)
+        const float d = v == -INFINITY ? -INFINITY : v - s.m, e = expf(d);
+        s.s += e;
+        s.t += e > 0.0f ? e * d : e;
+      });
+  if (kTop) {
+    // the c-th largest of this warp's lanes' maxima: warps c >= k of them, so at least k logits are not below the smallest of the
+    // warps' c-th
+    uint32_t key = ordered(s.m), cth = 0;
+    for (int i = (a.k + warps - 1) / warps; i > 0; i--) {
+      cth = __reduce_max_sync(0xffffffffu, key);
+      const unsigned who = __ballot_sync(0xffffffffu, key == cth);
+      if (lane == __ffs(who) - 1) key = 0;
+    }
+    if (lane == 0) bounds[wid] = cth;
+    if (threadIdx.x == 0) count = 0;
   }
+  auto joined = [&](Sums s) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      Sums x;
+      x.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+      x.s = __shfl_xor_sync(0xffffffffu, s.s, o);
+      x.t = __shfl_xor_sync(0xffffffffu, s.t, o);
+      s = (threadIdx.x & o) ? join(x, s) : join(s, x);       // (the same order in both lanes: the same bits)
+    }
+    return s;
+  };
+  s = joined(s);
   if (lane == 0) sums[wid] = s;
-  if (kTop && lane < a.k) lists[wid * kMostTop + lane] = top;
   __syncthreads();
-  if (wid) return;
-  s = lane < warps ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums x;
-    x.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-    x.s = __shfl_xor_sync(0xffffffffu, s.s, o);
-    x.t = __shfl_xor_sync(0xffffffffu, s.t, o);
-    s = (threadIdx.x & o) ? join(x, s) : join(s, x);
-  }
+  if (!kTop && wid) return;
+  s = joined(lane < warps ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f});
   const bool none = s.m == -INFINITY && s.s == s.s, bad = s.s != s.s;
   const float ls = none ? 0.0f : logf(s.s);
   const float nan = __int_as_float(0x7fc00000);
-  if (lane == 0) {
+  if (threadIdx.x == 0) {
     if (a.logp) {
       const int t = token_of(a.tokens[c], a.h);
       a.logp[c] = t < 0 || bad ? nan : none ? -INFINITY : (col[t] - s.m) - ls;
@@ -188,15 +206,53 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a) {
       a.stats[2 * c + 1] = bad ? nan : ls;
     }
   }
-  if (kTop) {
+  if constexpr (kTop) {
+    float *top = a.top + c * a.k, *number = a.top_tokens + c * a.k;
+    auto put = [&](int rank, const Top& x) {
+      top[rank] = none ? -INFINITY : (x.v - s.m) - ls;
+      number[rank] = (float)x.i;
+    };
+    if (bad) {
+      if (threadIdx.x < a.k) {
+        top[threadIdx.x] = nan;
+        number[threadIdx.x] = (float)threadIdx.x;
+      }
+      return;
+    }
+    // The column again (from L1 or L2): what is not below the bound, of all words that are left where the bound is -inf.
+    const float bound = unordered(__reduce_min_sync(0xffffffffu, lane < warps ? bounds[lane] : 0xffffffffu));
+    const bool open = bound == -INFINITY;
+    each([](float (&)[kBatch][kVec]) {},
+         [&](float v, int i) {
+           if (open ? v > bound : v >= bound && i != 0x7fffffff) {
+             const int at = atomicAdd(&count, 1);
+             if (at < kCandidates) candidates[at] = Top{v, i};
+           }
+         });
+    __syncthreads();
+    const int n = count;
+    if (n >= a.k && n <= kCandidates) {
+      for (int x = threadIdx.x; x < n; x += blockDim.x) {
+        const Top mine = candidates[x];
+        int rank = 0;
+        for (int y = 0; y < n; y++) rank += beats(candidates[y].v, candidates[y].i, mine.v, mine.i);
+        if (rank < a.k) put(rank, mine);
+      }
+      return;
+    }
+    // Too many (equal logits, a column in order) or too few: sorted lists.
+    Top list = {-INFINITY, 0x7fffffff};
+    float kv = -INFINITY;
+    int ki = 0x7fffffff;
+    each([](float (&)[kBatch][kVec]) {}, [&](float v, int i) { offer(list, a.k, v, i, kv, ki); });
+    if (lane < a.k) lists[wid * kMostTop + lane] = list;
+    __syncthreads();
+    if (wid) return;
     for (int x = 1; x < warps; x++) {
       const Top other = lane < a.k ? lists[x * kMostTop + lane] : Top{-INFINITY, 0x7fffffff};
-      offer(top, a.k, other.v, other.i, kv, ki);
+      offer(list, a.k, other.v, other.i, kv, ki);
     }
-    if (lane < a.k) {
-      a.top[c * a.k + lane] = bad ? nan : none ? -INFINITY : (top.v - s.m) - ls;
-      a.top_tokens[c * a.k + lane] = bad ? (float)lane : (float)top.i;
-    }
+    if (lane < a.k) put(lane, list);
   }
 }
 
