@@ -5,7 +5,8 @@
 // The logits are read once: every thread carries m, s and sum exp(d) d of what it has seen, joined by warps, then by the
 // block.  Bound by HBM (4 bytes a logit forward, 8 back).  For the k likeliest (k <= 32, equal logits by the lower number) the
 // threads' maxima give a bound that at least k logits reach and few others do: the column is read again, from L1 or L2, and
-// what reaches the bound is ranked (50 021 words of normal logits, k 20: about 60).  Where more than 512 do, or a mask leaves
+// what reaches the bound is ranked (50 021 words of normal logits, k 20: about 60).  Where more than 1024 do (128 where eight columns share a
+// block), or a mask leaves
 // fewer than k, sorted lists across the lanes of each warp find them, slowly where many logits rise above all before them.
 // A column whose logits are all -inf has no distribution: log p is -inf, H 0 and the gradient 0.  A NaN or +inf among a
 // column's logits makes all its results NaN (its likeliest tokens are then 0, 1, ...).
@@ -17,21 +18,39 @@ namespace {
 
 constexpr int kMostTop = 32;
 
+// Sums of powers of two: t is in units of log 2, which is multiplied in at the end.
 struct Sums {
-  float m, s, t;          // maximum, sum exp(z - m), sum exp(z - m) (z - m)
+  float m, s, t;          // maximum, sum exp(z - m), sum exp(z - m) (z - m) / log 2
 };
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.4028234e38f;
 
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// exp(x) for x <= 0, to two units in the last place whatever x is: what the product with log2 e rounds off is put back.
+__device__ __forceinline__ float exp_accurate(float x) {
+  const float y = x * kLog2e;
+  float r = fmaf(x, kLog2e, -y);
+  r = fmaf(x, 1.9259629911e-8f, r);
+  const float e = exp2_approx(y);
+  return y > -126.0f ? fmaf(e, r * kLn2, e) : e;
+}
+
+// The sums under a maximum of `m` (not below theirs).
+__device__ __forceinline__ void rescale(Sums& a, float m) {
+  const float d = (a.m - m) * kLog2e, f = exp2_approx(d);      // (a.m of -inf: 0, and its sums are 0 or NaN)
+  a.t = f > 0.0f ? (a.t + d * a.s) * f : 0.0f * a.s;
+  a.s *= f;
+  a.m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
   const float m = fmaxf(a.m, b.m);
   if (m == -INFINITY) return a.s != a.s ? a : b;             // (nothing but -inf, or NaN)
-  const float da = a.m - m, db = b.m - m;                    // one of them 0
-  const float fa = expf(da), fb = expf(db);
-  Sums r;
-  r.m = m;
-  r.s = a.s * fa + b.s * fb;
-  r.t = fa > 0.0f ? (a.t + da * a.s) * fa : 0.0f * a.s;      // (0 * s: NaN stays)
-  r.t += fb > 0.0f ? (b.t + db * b.s) * fb : 0.0f * b.s;
-  return r;
+  rescale(a, m);
+  rescale(b, m);
+  return Sums{m, a.s + b.s, a.t + b.t};
 }
 
 // The list a warp keeps: lane i holds the i-th likeliest so far.
@@ -103,30 +122,36 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 }
 __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-constexpr int kCandidates = 512;
+constexpr int kCandidates = 1024;      // of a block's columns together
 
-// kBatch groups of kVec logits of a thread, all read before the first is used.
+// A column is read by `warps` of the block's warps (a power of two), kBatch groups of kVec logits of a thread before the first is
+// used.
 template <int kVec, bool kTop>
-__global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a) {
+__global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warps) {
   constexpr int kBatch = kVec == 4 ? 2 : 8;
   __shared__ Sums sums[32];
   __shared__ uint32_t bounds[32];
   __shared__ Top lists[kTop ? 32 * kMostTop : 1], candidates[kTop ? kCandidates : 1];
-  __shared__ int count;
+  __shared__ int counts[32];
   grid_dependents_launch();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const long c = blockIdx.x;
+  const int threads = 32 * warps, group = threadIdx.x / threads, groups = blockDim.x / threads, t = threadIdx.x % threads;
+  const int lane = threadIdx.x & 31, wid = t >> 5, first_warp = group * warps;
+  const long c = (long)blockIdx.x * groups + group;
+  if (c >= a.w) return;                                // (a column's threads together: nobody waits for them)
   const float* col = a.z + c * a.h;
-  Sums s = {-INFINITY, 0.0f, 0.0f};
   const int items = a.h / kVec;                        // (kVec 4: h is a multiple)
-  // f(value, its number) for every logit of this thread (-inf, 0x7fffffff beyond the last); all threads of a block go round together
+  auto meet = [&]() {
+    if (warps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads) : "memory");
+  };
+  // before(values of a batch), then f(value, its number) for each if it wants them; -inf beyond the last
   auto each = [&](auto before, auto f) {
-    for (int base = 0; base < items; base += kBatch * (int)blockDim.x) {
+    for (int base = 0; base < items; base += kBatch * threads) {
       float v[kBatch][kVec];
 #pragma unroll
       for (int b = 0; b < kBatch; b++) {
-        const int i = base + b * (int)blockDim.x + (int)threadIdx.x;
+        const int i = base + b * threads + t;
         if (i < items) {
           load<kVec>(col, i, v[b]);
         } else {
@@ -134,35 +159,32 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a) {
           for (int j = 0; j < kVec; j++) v[b][j] = -INFINITY;
         }
       }
-      before(v);
+      float m = -INFINITY;
 #pragma unroll
       for (int b = 0; b < kBatch; b++)
 #pragma unroll
-        for (int j = 0; j < kVec; j++) {
-          const int i = base + b * (int)blockDim.x + (int)threadIdx.x;
-          f(v[b][j], i < items ? kVec * i + j : 0x7fffffff);
-        }
+        for (int j = 0; j < kVec; j++) m = fmaxf(m, v[b][j]);
+      if (!before(m)) continue;
+#pragma unroll
+      for (int b = 0; b < kBatch; b++)
+#pragma unroll
+        for (int j = 0; j < kVec; j++) f(v[b][j], kVec * (base + b * threads + t) + j);
     }
   };
+  Sums s = {-INFINITY, 0.0f, 0.0f};
+  float m = kLowest;                                   // s.m, finite where nothing but -inf was seen
   each(
-      [&](float (&v)[kBatch][kVec]) {
-        float m = s.m;
-#pragma unroll
-        for (int b = 0; b < kBatch; b++)
-#pragma unroll
-          for (int j = 0; j < kVec; j++) m = fmaxf(m, v[b][j]);
-        if (m > s.m) {
-          const float d = s.m - m, f = expf(d);
-          s.t = f > 0.0f ? (s.t + d * s.s) * f : 0.0f * s.s;
-          s.s *= f;
-          s.m = m;
+      [&](float best) {
+        if (best > s.m) {
+          rescale(s, best);
+          m = fmaxf(best, kLowest);
         }
+        return true;
       },
       [&](float v, int) {
-        // (a maximum of -inf: nothing to add but a NaN)
-        const float d = v == -INFINITY ? -INFINITY : v - s.m, e = expf(d);
+        const float d = (v - m) * kLog2e, e = exp2_approx(d);
         s.s += e;
-        s.t += e > 0.0f ? e * d : e;
+        s.t = fmaf(e, fmaxf(d, -200.0f), s.t);         // (2^-200 is 0 here: no 0 x inf)
       });
   if (kTop) {
     // the c-th largest of this warp's lanes' maxima: warps c >= k of them, so at least k logits are not below the smallest of the
@@ -173,8 +195,8 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a) {
       const unsigned who = __ballot_sync(0xffffffffu, key == cth);
       if (lane == __ffs(who) - 1) key = 0;
     }
-    if (lane == 0) bounds[wid] = cth;
-    if (threadIdx.x == 0) count = 0;
+    if (lane == 0) bounds[first_warp + wid] = cth;
+    if (t == 0) counts[group] = 0;
   }
   auto joined = [&](Sums s) {
 #pragma unroll
@@ -183,24 +205,28 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a) {
       x.m = __shfl_xor_sync(0xffffffffu, s.m, o);
       x.s = __shfl_xor_sync(0xffffffffu, s.s, o);
       x.t = __shfl_xor_sync(0xffffffffu, s.t, o);
-      s = (threadIdx.x & o) ? join(x, s) : join(s, x);       // (the same order in both lanes: the same bits)
+      s = (lane & o) ? join(x, s) : join(s, x);              // (the same order in both lanes: the same bits)
     }
     return s;
   };
   s = joined(s);
-  if (lane == 0) sums[wid] = s;
-  __syncthreads();
-  if (!kTop && wid) return;
-  s = joined(lane < warps ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f});
+  if (warps > 1) {
+    if (lane == 0) sums[first_warp + wid] = s;
+    meet();
+    if (!kTop && wid) return;
+    s = joined(lane < warps ? sums[first_warp + lane] : Sums{-INFINITY, 0.0f, 0.0f});
+  } else if (kTop) {
+    meet();
+  }
   const bool none = s.m == -INFINITY && s.s == s.s, bad = s.s != s.s;
   const float ls = none ? 0.0f : logf(s.s);
   const float nan = __int_as_float(0x7fc00000);
-  if (threadIdx.x == 0) {
+  if (t == 0) {
     if (a.logp) {
-      const int t = token_of(a.tokens[c], a.h);
-      a.logp[c] = t < 0 || bad ? nan : none ? -INFINITY : (col[t] - s.m) - ls;
+      const int w = token_of(a.tokens[c], a.h);
+      a.logp[c] = w < 0 || bad ? nan : none ? -INFINITY : (col[w] - s.m) - ls;
     }
-    if (a.entropy) a.entropy[c] = bad ? nan : none ? 0.0f : ls - s.t / s.s;
+    if (a.entropy) a.entropy[c] = bad ? nan : none ? 0.0f : ls - s.t * kLn2 / s.s;
     if (a.stats) {
       a.stats[2 * c] = bad ? nan : s.m;
       a.stats[2 * c + 1] = bad ? nan : ls;
@@ -213,43 +239,44 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a) {
       number[rank] = (float)x.i;
     };
     if (bad) {
-      if (threadIdx.x < a.k) {
-        top[threadIdx.x] = nan;
-        number[threadIdx.x] = (float)threadIdx.x;
+      if (t < a.k) {
+        top[t] = nan;
+        number[t] = (float)t;
       }
       return;
     }
-    // The column again (from L1 or L2): what is not below the bound, of all words that are left where the bound is -inf.
-    const float bound = unordered(__reduce_min_sync(0xffffffffu, lane < warps ? bounds[lane] : 0xffffffffu));
-    const bool open = bound == -INFINITY;
-    each([](float (&)[kBatch][kVec]) {},
+    // The column again (from L1 or L2): what is not below the bound; all words that are left where the bound is -inf.
+    const float bound = fmaxf(unordered(__reduce_min_sync(0xffffffffu, lane < warps ? bounds[first_warp + lane] : 0xffffffffu)), kLowest);
+    const int room = kCandidates / groups;
+    Top* found = candidates + group * room;
+    each([&](float best) { return best >= bound; },
          [&](float v, int i) {
-           if (open ? v > bound : v >= bound && i != 0x7fffffff) {
-             const int at = atomicAdd(&count, 1);
-             if (at < kCandidates) candidates[at] = Top{v, i};
+           if (v >= bound) {
+             const int at = atomicAdd(&counts[group], 1);
+             if (at < room) found[at] = Top{v, i};
            }
          });
-    __syncthreads();
-    const int n = count;
-    if (n >= a.k && n <= kCandidates) {
-      for (int x = threadIdx.x; x < n; x += blockDim.x) {
-        const Top mine = candidates[x];
+    meet();
+    const int n = counts[group];
+    if (n >= a.k && n <= room) {
+      for (int x = t; x < n; x += threads) {
+        const Top mine = found[x];
         int rank = 0;
-        for (int y = 0; y < n; y++) rank += beats(candidates[y].v, candidates[y].i, mine.v, mine.i);
+        for (int y = 0; y < n; y++) rank += beats(found[y].v, found[y].i, mine.v, mine.i);
         if (rank < a.k) put(rank, mine);
       }
       return;
     }
-    // Too many (equal logits, a column in order) or too few: sorted lists.
+    // Too many (equal logits, a column in order) or too few: sorted lists.  (An item beyond the last beats nothing.)
     Top list = {-INFINITY, 0x7fffffff};
     float kv = -INFINITY;
     int ki = 0x7fffffff;
-    each([](float (&)[kBatch][kVec]) {}, [&](float v, int i) { offer(list, a.k, v, i, kv, ki); });
-    if (lane < a.k) lists[wid * kMostTop + lane] = list;
-    __syncthreads();
+    each([](float) { return true; }, [&](float v, int i) { offer(list, a.k, v, i < a.h ? i : 0x7fffffff, kv, ki); });
+    if (lane < a.k) lists[(first_warp + wid) * kMostTop + lane] = list;
+    meet();
     if (wid) return;
     for (int x = 1; x < warps; x++) {
-      const Top other = lane < a.k ? lists[x * kMostTop + lane] : Top{-INFINITY, 0x7fffffff};
+      const Top other = lane < a.k ? lists[(first_warp + x) * kMostTop + lane] : Top{-INFINITY, 0x7fffffff};
       offer(list, a.k, other.v, other.i, kv, ki);
     }
     if (lane < a.k) put(lane, list);
@@ -287,7 +314,7 @@ __global__ void __launch_bounds__(256) k_log_prob_deriv(const float* z, const fl
       for (int j = 0; j < kVec; j++) {
         float r = 0.0f;
         if (!zero) {
-          const float lp = (v[b][j] - m) - ls, p = expf(lp);
+          const float lp = (v[b][j] - m) - ls, p = exp_accurate(lp);
           // -p (g + q (log p + H)), and 0 where p is: log p may be -inf there
           r = p > 0.0f ? -p * (g + q * (lp + H)) : 0.0f * p;
           if (kVec * i + j == t) r += g;
@@ -347,7 +374,9 @@ int log_prob(cudamat* logits, cudamat* tokens, cudamat* target, cudamat* entropy
   // as many warps a column as fill the device, with eight logits a thread or more
   int warps = 1;
   while (warps < 32 && (long)w * warps < 32L * sm_count() && (long)warps * 32 * 8 < h) warps *= 2;
-#define LOGP(VEC, TOP) (void)launch_dependent(k_log_prob<VEC, TOP>, dim3(w), dim3(32 * warps), 0, stream(), a)
+  const int groups = warps < 8 ? 8 / warps : 1;          // columns of a block
+#define LOGP(VEC, TOP) \
+  (void)launch_dependent(k_log_prob<VEC, TOP>, dim3((w + groups - 1) / groups), dim3(32 * warps * groups), 0, stream(), a, warps)
   if (vec && a.k) LOGP(4, true);
   else if (vec) LOGP(4, false);
   else if (a.k) LOGP(1, true);
