@@ -128,7 +128,7 @@ constexpr int kCandidates = 1024;      // of a block's columns together
 // used.
 template <int kVec, bool kTop>
 __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warps) {
-  constexpr int kBatch = kVec == 4 ? 2 : 8;
+  constexpr int kBatch = 16 / kVec;
   __shared__ Sums sums[32];
   __shared__ uint32_t bounds[32];
   __shared__ Top lists[kTop ? 32 * kMostTop : 1], candidates[kTop ? kCandidates : 1];
@@ -143,7 +143,11 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
   const int items = a.h / kVec;                        // (kVec 4: h is a multiple)
   auto meet = [&]() {
     if (warps == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads) : "memory");
+    else if (groups == 1) __syncthreads();
+    else if (group == 0) asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+    else if (group == 1) asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory");
+    else if (group == 2) asm volatile("bar.sync 3, %0;" ::"r"(threads) : "memory");
+    else asm volatile("bar.sync 4, %0;" ::"r"(threads) : "memory");      // (at most four columns of two warps or more)
   };
   // before(values of a batch), then f(value, its number) for each if it wants them; -inf beyond the last
   auto each = [&](auto before, auto f) {
@@ -371,10 +375,17 @@ int log_prob(cudamat* logits, cudamat* tokens, cudamat* target, cudamat* entropy
   a.w = w;
   a.k = top ? top->size[0] : 0;
   const bool vec = h % 4 == 0 && on16(a.z);
-  // as many warps a column as fill the device, with eight logits a thread or more
+  // as many warps a column as fill the device, with sixteen logits a thread or more
   int warps = 1;
-  while (warps < 32 && (long)w * warps < 32L * sm_count() && (long)warps * 32 * 8 < h) warps *= 2;
+  while (warps < 32 && (long)w * warps < 32L * sm_count() && (long)warps * 32 * 16 < h) warps *= 2;
   const int groups = warps < 8 ? 8 / warps : 1;          // columns of a block
+  // (room for as many blocks as the registers allow: left to itself the runtime may give shared memory less)
+  static const bool carved = [] {
+    for (auto kernel : {k_log_prob<1, false>, k_log_prob<4, false>, k_log_prob<1, true>, k_log_prob<4, true>})
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 50) != cudaSuccess) cudaGetLastError();
+    return true;
+  }();
+  (void)carved;
 #define LOGP(VEC, TOP) \
   (void)launch_dependent(k_log_prob<VEC, TOP>, dim3((w + groups - 1) / groups), dim3(32 * warps * groups), 0, stream(), a, warps)
   if (vec && a.k) LOGP(4, true);

@@ -53,7 +53,7 @@ def norm_exact(x, gain, bias, eps):
 
 
 SHAPES = [(1, 1), (1, 7), (3, 5), (31, 9), (32, 1), (33, 2), (64, 17), (100, 100), (128, 3), (257, 31), (500, 8), (512, 40), (513, 12),
-          (784, 100), (1024, 33), (1028, 5), (1357, 203), (2048, 64), (4096, 50), (4100, 3), (4099, 20), (8192, 9), (8195, 4),
+          (784, 100), (510, 700), (1023, 900), (2047, 1300), (8190, 700), (1024, 33), (1028, 5), (1357, 203), (2048, 64), (4096, 50), (4100, 3), (4099, 20), (8192, 9), (8195, 4),
           (16384, 3), (20000, 5), (32772, 2), (40001, 3), (500, 3001), (16, 4096)]
 
 
@@ -129,6 +129,27 @@ def test_layer_norm_of_matrices_that_start_anywhere(cm, off):
     for a, b in ((out, want), (dx, wdx)):
         np.testing.assert_allclose(get(a), get(b), rtol=0, atol=2 * 45 * U * 20)
     np.testing.assert_allclose(get(gg), get(wg), rtol=0, atol=2 * (45 + 37) * U * 21 * 20)
+
+
+@pytest.mark.parametrize("shape", [(37, 50), (1001, 23), (1024, 30), (9001, 3)])
+def test_layer_norm_of_matrices_that_lie_differently(cm, shape):
+    """Inputs, gradients and results at different distances from 16 bytes."""
+    h, w = shape
+    rng = np.random.default_rng(h)
+    x, dy = (rng.standard_normal(shape).astype(np.float32) for _ in range(2))
+    z = np.zeros_like(x)
+    want, wdx, wst, wg = cm.empty(shape), cm.empty(shape), cm.empty((2, w)), cm.empty((h, 1))
+    cm.CUDAMatrix(x).layer_norm(target=want, stats=wst)
+    cm.CUDAMatrix(dy).layer_norm_deriv(cm.CUDAMatrix(x), wst, target=wdx, grad_gain=wg)
+    for a, b, c in ((1, 0, 0), (0, 2, 0), (0, 0, 3), (1, 2, 3)):
+        gx, out, dx = odd_start(cm, x, a), odd_start(cm, z, b), odd_start(cm, z, c)
+        st, gg = cm.empty((2, w)), cm.empty((h, 1))
+        gx.layer_norm(target=out, stats=st)
+        odd_start(cm, dy, b).layer_norm_deriv(gx, st, target=dx, grad_gain=gg)
+        n = max(32, -(-h // 1024)) + 12          # as in norm_exact, twice: two groupings of sums of values up to 6
+        np.testing.assert_allclose(get(out), get(want), rtol=0, atol=2 * n * U * 20)
+        np.testing.assert_allclose(get(dx), get(wdx), rtol=0, atol=2 * n * U * 20)
+        np.testing.assert_allclose(get(gg), get(wg), rtol=0, atol=2 * (n + w + 16) * U * w * 20)
 
 
 def test_layer_norm_of_constant_and_extreme_columns(cm):
