@@ -99,20 +99,26 @@ __device__ __forceinline__ int token_of(float f, int n) {
   return i < 0 || i >= n ? -1 : i;
 }
 
-// Group i of kVec logits (4: on 16 bytes).
-template <int kVec>
-__device__ __forceinline__ void load(const float* p, long i, float (&v)[kVec]) {
-  if constexpr (kVec == 4) {
-    const float4 x = reinterpret_cast<const float4*>(p)[i];
+// A column in groups of four values on 16 bytes, wherever it starts: group q holds rows 4 q - o .. of a column that starts o floats
+// behind a 16-byte boundary; only the first and the last may be partial.  (Value by value 9999 x 4096 takes 44 us, so 35.)
+__device__ __forceinline__ int offset_in(const float* column) { return (int)((uintptr_t)column >> 2 & 3); }
+__device__ __forceinline__ void load_group(const float* column, int r, int h, float none, float (&v)[4]) {
+  if (r >= 0 && r + 4 <= h) {
+    const float4 x = *reinterpret_cast<const float4*>(column + r);
     v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
   } else {
-    v[0] = p[i];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = r + j >= 0 && r + j < h ? column[r + j] : none;
   }
 }
-template <int kVec>
-__device__ __forceinline__ void store(float* p, long i, const float (&v)[kVec]) {
-  if constexpr (kVec == 4) reinterpret_cast<float4*>(p)[i] = make_float4(v[0], v[1], v[2], v[3]);
-  else p[i] = v[0];
+__device__ __forceinline__ void store_group(float* column, int r, int h, const float (&v)[4]) {
+  if (r >= 0 && r + 4 <= h) {
+    *reinterpret_cast<float4*>(column + r) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (r + j >= 0 && r + j < h) column[r + j] = v[j];
+  }
 }
 
 // A float's bits in the floats' order, and back (0: below all).
@@ -124,11 +130,11 @@ __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(
 
 constexpr int kCandidates = 1024;      // of a block's columns together
 
-// A column is read by `warps` of the block's warps (a power of two), kBatch groups of kVec logits of a thread before the first is
-// used.
-template <int kVec, bool kTop>
+// A column is read by `warps` of the block's warps (a power of two), the next kBatch groups of a thread on their way while it works
+// on some.
+template <bool kTop>
 __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warps) {
-  constexpr int kBatch = 16 / kVec;
+  constexpr int kBatch = 4;
   __shared__ Sums sums[32];
   __shared__ uint32_t bounds[32];
   __shared__ Top lists[kTop ? 32 * kMostTop : 1], candidates[kTop ? kCandidates : 1];
@@ -140,7 +146,7 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
   const long c = (long)blockIdx.x * groups + group;
   if (c >= a.w) return;                                // (a column's threads together: nobody waits for them)
   const float* col = a.z + c * a.h;
-  const int items = a.h / kVec;                        // (kVec 4: h is a multiple)
+  const int o = offset_in(col), items = (a.h + o + 3) >> 2;
   auto meet = [&]() {
     if (warps == 1) __syncwarp();
     else if (groups == 1) __syncthreads();
@@ -151,28 +157,37 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
   };
   // before(values of a batch), then f(value, its number) for each if it wants them; -inf beyond the last
   auto each = [&](auto before, auto f) {
-    for (int base = 0; base < items; base += kBatch * threads) {
-      float v[kBatch][kVec];
+    float next[kBatch][4];
+    auto fetch = [&](int base) {
 #pragma unroll
       for (int b = 0; b < kBatch; b++) {
         const int i = base + b * threads + t;
         if (i < items) {
-          load<kVec>(col, i, v[b]);
+          load_group(col, 4 * i - o, a.h, -INFINITY, next[b]);
         } else {
 #pragma unroll
-          for (int j = 0; j < kVec; j++) v[b][j] = -INFINITY;
+          for (int j = 0; j < 4; j++) next[b][j] = -INFINITY;
         }
       }
+    };
+    fetch(0);
+    for (int base = 0; base < items; base += kBatch * threads) {
+      float v[kBatch][4];
+#pragma unroll
+      for (int b = 0; b < kBatch; b++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[b][j] = next[b][j];
+      fetch(base + kBatch * threads);                  // on its way while this batch is worked on
       float m = -INFINITY;
 #pragma unroll
       for (int b = 0; b < kBatch; b++)
 #pragma unroll
-        for (int j = 0; j < kVec; j++) m = fmaxf(m, v[b][j]);
+        for (int j = 0; j < 4; j++) m = fmaxf(m, v[b][j]);
       if (!before(m)) continue;
 #pragma unroll
       for (int b = 0; b < kBatch; b++)
 #pragma unroll
-        for (int j = 0; j < kVec; j++) f(v[b][j], kVec * (base + b * threads + t) + j);
+        for (int j = 0; j < 4; j++) f(v[b][j], 4 * (base + b * threads + t) + j - o);
     }
   };
   Sums s = {-INFINITY, 0.0f, 0.0f};
@@ -275,7 +290,7 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
     Top list = {-INFINITY, 0x7fffffff};
     float kv = -INFINITY;
     int ki = 0x7fffffff;
-    each([](float) { return true; }, [&](float v, int i) { offer(list, a.k, v, i < a.h ? i : 0x7fffffff, kv, ki); });
+    each([](float) { return true; }, [&](float v, int i) { offer(list, a.k, v, i >= 0 && i < a.h ? i : 0x7fffffff, kv, ki); });
     if (lane < a.k) lists[(first_warp + wid) * kMostTop + lane] = list;
     meet();
     if (wid) return;
@@ -287,46 +302,51 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
   }
 }
 
-// grid.x: columns; grid.y: parts of a column.  A column without weight is not read.
-template <int kVec>
+// `warps` of a block's eight warps a column, grid.y parts of it.  A column without weight is not read.  kAlike: logits and gradient
+// lie the same way to 16 bytes.
+template <bool kAlike>
 __global__ void __launch_bounds__(256) k_log_prob_deriv(const float* z, const float* tokens, const float* stats, const float* grad,
-                                                        const float* entropy, const float* grad_entropy, float* dz, int h) {
-  constexpr int kBatch = kVec == 4 ? 2 : 8;
+                                                        const float* entropy, const float* grad_entropy, float* dz, int h, int w, int warps) {
+  constexpr int kBatch = kAlike ? 2 : 8, kValues = kAlike ? 4 : 1;
   grid_dependents_launch();
   grid_dependency_wait();
-  const long c = blockIdx.x;
+  const int threads = 32 * warps;
+  const long c = (long)blockIdx.x * (8 / warps) + threadIdx.x / threads;
+  if (c >= w) return;
   const float g = grad ? grad[c] : 0.0f, q = grad_entropy ? grad_entropy[c] : 0.0f, H = grad_entropy ? entropy[c] : 0.0f;
   const float m = stats[2 * c], ls = stats[2 * c + 1];
   const int t = g != 0.0f ? token_of(tokens[c], h) : -1;
   const bool zero = (g == 0.0f && q == 0.0f) || m == -INFINITY, bad = g != 0.0f && t < 0;
   const float* col = z + c * h;
   float* out = dz + c * h;
-  const int items = h / kVec, step = gridDim.y * blockDim.x;
-  for (int base = blockIdx.y * blockDim.x + threadIdx.x; base < items; base += kBatch * step) {
-    float v[kBatch][kVec];
+  const int o = kAlike ? offset_in(col) : 0, items = kAlike ? (h + o + 3) >> 2 : h, step = gridDim.y * threads;
+  for (int base = blockIdx.y * threads + threadIdx.x % threads; base < items; base += kBatch * step) {
+    float v[kBatch][kValues];
 #pragma unroll
     for (int b = 0; b < kBatch; b++) {
       const int i = base + b * step;
       if (zero || i >= items) continue;
-      load<kVec>(col, i, v[b]);
+      if constexpr (kAlike) load_group(col, 4 * i - o, h, 0.0f, v[b]);
+      else v[b][0] = col[i];
     }
 #pragma unroll
     for (int b = 0; b < kBatch; b++) {
       const int i = base + b * step;
       if (i >= items) continue;
 #pragma unroll
-      for (int j = 0; j < kVec; j++) {
+      for (int j = 0; j < kValues; j++) {
         float r = 0.0f;
         if (!zero) {
           const float lp = (v[b][j] - m) - ls, p = exp_accurate(lp);
           // -p (g + q (log p + H)), and 0 where p is: log p may be -inf there
           r = p > 0.0f ? -p * (g + q * (lp + H)) : 0.0f * p;
-          if (kVec * i + j == t) r += g;
+          if (kValues * i + j - o == t) r += g;
           if (bad) r = __int_as_float(0x7fc00000);
         }
         v[b][j] = r;
       }
-      store<kVec>(out, i, v[b]);
+      if constexpr (kAlike) store_group(out, 4 * i - o, h, v[b]);
+      else out[i] = v[b][0];
     }
   }
 }
@@ -337,7 +357,6 @@ int row_ok(const cudamat* v, int w) {
   if (!v->on_device) return ERROR_NOT_ON_DEVICE;
   return v->size[0] == 1 && v->size[1] == w ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
 }
-bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
@@ -374,25 +393,12 @@ int log_prob(cudamat* logits, cudamat* tokens, cudamat* target, cudamat* entropy
   a.h = h;
   a.w = w;
   a.k = top ? top->size[0] : 0;
-  const bool vec = h % 4 == 0 && on16(a.z);
   // as many warps a column as fill the device, with sixteen logits a thread or more
   int warps = 1;
   while (warps < 32 && (long)w * warps < 32L * sm_count() && (long)warps * 32 * 16 < h) warps *= 2;
   const int groups = warps < 8 ? 8 / warps : 1;          // columns of a block
-  // (room for as many blocks as the registers allow: left to itself the runtime may give shared memory less)
-  static const bool carved = [] {
-    for (auto kernel : {k_log_prob<1, false>, k_log_prob<4, false>, k_log_prob<1, true>, k_log_prob<4, true>})
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 50) != cudaSuccess) cudaGetLastError();
-    return true;
-  }();
-  (void)carved;
-#define LOGP(VEC, TOP) \
-  (void)launch_dependent(k_log_prob<VEC, TOP>, dim3((w + groups - 1) / groups), dim3(32 * warps * groups), 0, stream(), a, warps)
-  if (vec && a.k) LOGP(4, true);
-  else if (vec) LOGP(4, false);
-  else if (a.k) LOGP(1, true);
-  else LOGP(1, false);
-#undef LOGP
+  (void)launch_dependent(a.k ? k_log_prob<true> : k_log_prob<false>, dim3((w + groups - 1) / groups), dim3(32 * warps * groups), 0, stream(),
+                         a, warps);
   return check_launch();
 }
 
@@ -412,17 +418,15 @@ int log_prob_deriv(cudamat* logits, cudamat* tokens, cudamat* stats, cudamat* gr
   auto at = [](cudamat* v) { return v ? v->data_device : nullptr; };
   const float* z = logits->data_device;
   float* dz = target->data_device;
-  const bool vec = h % 4 == 0 && on16(z) && on16(dz);
+  // a warp a column up to 256 logits, a block from 1024 on, and parts of a column where there are few
+  int warps = 1;
+  while (warps < 8 && warps * 256 < h) warps *= 2;
   const int per_block = 256 * 8;                         // logits of a block's batch
   int parts = (h + per_block - 1) / per_block;
   while (parts > 1 && (long)w * parts > 16L * sm_count()) parts = (parts + 1) / 2;
-  const dim3 grid(w, parts);
-  if (vec)
-    (void)launch_dependent(k_log_prob_deriv<4>, grid, dim3(256), 0, stream(), z, at(tokens), stats->data_device, at(grad), at(entropy),
-                           at(grad_entropy), dz, h);
-  else
-    (void)launch_dependent(k_log_prob_deriv<1>, grid, dim3(256), 0, stream(), z, at(tokens), stats->data_device, at(grad), at(entropy),
-                           at(grad_entropy), dz, h);
+  const dim3 grid((w + 8 / warps - 1) / (8 / warps), parts);
+  (void)launch_dependent(((uintptr_t)z & 15) == ((uintptr_t)dz & 15) ? k_log_prob_deriv<true> : k_log_prob_deriv<false>, grid, dim3(256), 0,
+                         stream(), z, at(tokens), stats->data_device, at(grad), at(entropy), at(grad_entropy), dz, h, w, warps);
   return check_launch();
 }
 

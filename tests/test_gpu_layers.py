@@ -402,6 +402,20 @@ def test_logits_that_start_anywhere(cm, off):
         np.testing.assert_allclose(x, y, rtol=0, atol=2 * 60 * U * 12)
 
 
+@pytest.mark.parametrize("h", [7, 300, 2049])
+def test_logits_and_gradient_that_lie_differently(cm, h):
+    rng = np.random.default_rng(h)
+    z = rng.standard_normal((h, 11)).astype(np.float32)
+    gz, t, g = cm.CUDAMatrix(z), cm.CUDAMatrix(rng.integers(0, h, (1, 11)).astype(np.float32)), cm.CUDAMatrix(rng.standard_normal((1, 11)))
+    st, want = cm.empty((2, 11)), cm.empty((h, 11))
+    gz.log_prob(t, stats=st)
+    gz.log_prob_deriv(t, st, g, target=want)
+    for off in (1, 2, 3):                      # elementwise: the same bits
+        got = odd_start(cm, np.zeros_like(z), off)
+        gz.log_prob_deriv(t, st, g, target=got)
+        assert np.array_equal(get(got), get(want))
+
+
 # -- streams and graphs -------------------------------------------------------------------------
 class _On(object):
     """The library's calls on a stream of torch's; with a graph, recorded."""
