@@ -4,8 +4,8 @@
 //   dz_i = g (1[i = t] - p_i) - q p_i (log p_i + H)      for gradients g of log p_t and q of H
 // The logits are read once: every thread carries m, s and sum exp(d) d of what it has seen, joined by warps, then by the
 // block.  Bound by HBM (4 bytes a logit forward, 8 back).  For the k likeliest (k <= 32, equal logits by the lower number) the
-// threads' maxima give a bound that at least k logits reach and few others do: the column is read again, from L1 or L2, and
-// what reaches the bound is ranked (50 021 words of normal logits, k 20: about 60).  Where more than 1024 do (128 where eight columns share a
+// threads' maxima give a bound that at least k logits reach and few others do; the chunks of 128 logits whose maximum reaches it are
+// read again and what reaches it is ranked (50 021 words of normal logits, k 20: about 60).  Where more than 512 do (64 where eight columns share a
 // block), or a mask leaves
 // fewer than k, sorted lists across the lanes of each warp find them, slowly where many logits rise above all before them.
 // A column whose logits are all -inf has no distribution: log p is -inf, H 0 and the gradient 0.  A NaN or +inf among a
@@ -128,7 +128,8 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 }
 __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-constexpr int kCandidates = 1024;      // of a block's columns together
+constexpr int kCandidates = 512;       // of a block's columns together
+constexpr int kChunks = 2048;          // chunks (a warp's 128 logits) whose maxima a block keeps
 
 // A column is read by `warps` of the block's warps (a power of two), the next kBatch groups of a thread on their way while it works
 // on some.
@@ -137,7 +138,12 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
   constexpr int kBatch = 4;
   __shared__ Sums sums[32];
   __shared__ uint32_t bounds[32];
-  __shared__ Top lists[kTop ? 32 * kMostTop : 1], candidates[kTop ? kCandidates : 1];
+  // (the lists come after the maxima's last use)
+  __shared__ union {
+    uint32_t maxima[kTop ? kChunks : 1];
+    Top lists[kTop ? 32 * kMostTop : 1];
+  } shared;
+  __shared__ Top candidates[kTop ? kCandidates : 1];
   __shared__ int counts[32];
   grid_dependents_launch();
   grid_dependency_wait();
@@ -183,21 +189,31 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
       for (int b = 0; b < kBatch; b++)
 #pragma unroll
         for (int j = 0; j < 4; j++) m = fmaxf(m, v[b][j]);
-      if (!before(m)) continue;
+      if (!before(m, v, base)) continue;
 #pragma unroll
       for (int b = 0; b < kBatch; b++)
 #pragma unroll
         for (int j = 0; j < 4; j++) f(v[b][j], 4 * (base + b * threads + t) + j - o);
     }
   };
+  // this warp's chunks' maxima: chunk b of its round i at maxima[(i * kBatch + b) * warps + wid]
+  const int most = kChunks / groups;
+  uint32_t* const maxima = shared.maxima + (kTop ? group * most : 0);
+  const bool kept = ((items + kBatch * threads - 1) / (kBatch * threads)) * kBatch * warps <= most;
   Sums s = {-INFINITY, 0.0f, 0.0f};
   float m = kLowest;                                   // s.m, finite where nothing but -inf was seen
   each(
-      [&](float best) {
+      [&](float best, const float (&v)[kBatch][4], int base) {
         if (best > s.m) {
           rescale(s, best);
           m = fmaxf(best, kLowest);
         }
+        if (kTop && kept)
+#pragma unroll
+          for (int b = 0; b < kBatch; b++) {
+            const uint32_t of_chunk = __reduce_max_sync(0xffffffffu, ordered(fmaxf(fmaxf(v[b][0], v[b][1]), fmaxf(v[b][2], v[b][3]))));
+            if (lane == 0) maxima[base / 32 + b * warps + wid] = of_chunk;
+          }
         return true;
       },
       [&](float v, int) {
@@ -264,17 +280,37 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
       }
       return;
     }
-    // The column again (from L1 or L2): what is not below the bound; all words that are left where the bound is -inf.
+    // The column again (from L1 or L2), where a chunk's maximum says so: what is not below the bound; all words that are left where the
+    // bound is -inf.
     const float bound = fmaxf(unordered(__reduce_min_sync(0xffffffffu, lane < warps ? bounds[first_warp + lane] : 0xffffffffu)), kLowest);
     const int room = kCandidates / groups;
     Top* found = candidates + group * room;
-    each([&](float best) { return best >= bound; },
-         [&](float v, int i) {
-           if (v >= bound) {
-             const int at = atomicAdd(&counts[group], 1);
-             if (at < room) found[at] = Top{v, i};
-           }
-         });
+    auto offer_found = [&](float v, int i) {
+      if (v >= bound) {
+        const int at = atomicAdd(&counts[group], 1);
+        if (at < room) found[at] = Top{v, i};
+      }
+    };
+    if (kept) {
+      __syncwarp();                                    // (this warp's own maxima)
+      const uint32_t least = ordered(bound);
+      const int rounds = (items + threads - 1) / threads;
+      for (int first = 0; first < rounds; first += 32) {       // 32 of the warp's chunks at a time, those wanted one by one
+        unsigned wanted = __ballot_sync(0xffffffffu, first + lane < rounds && maxima[(first + lane) * warps + wid] >= least);
+        while (wanted) {
+          const int i = (first + __ffs(wanted) - 1) * threads + t;
+          wanted &= wanted - 1;
+          if (i < items) {
+            float v[4];
+            load_group(col, 4 * i - o, a.h, -INFINITY, v);
+#pragma unroll
+            for (int j = 0; j < 4; j++) offer_found(v[j], 4 * i + j - o);
+          }
+        }
+      }
+    } else {
+      each([&](float best, const float (&)[kBatch][4], int) { return best >= bound; }, offer_found);
+    }
     meet();
     const int n = counts[group];
     if (n >= a.k && n <= room) {
@@ -290,12 +326,12 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
     Top list = {-INFINITY, 0x7fffffff};
     float kv = -INFINITY;
     int ki = 0x7fffffff;
-    each([](float) { return true; }, [&](float v, int i) { offer(list, a.k, v, i >= 0 && i < a.h ? i : 0x7fffffff, kv, ki); });
-    if (lane < a.k) lists[(first_warp + wid) * kMostTop + lane] = list;
+    each([](float, const float (&)[kBatch][4], int) { return true; }, [&](float v, int i) { offer(list, a.k, v, i >= 0 && i < a.h ? i : 0x7fffffff, kv, ki); });
+    if (lane < a.k) shared.lists[(first_warp + wid) * kMostTop + lane] = list;
     meet();
     if (wid) return;
     for (int x = 1; x < warps; x++) {
-      const Top other = lane < a.k ? lists[(first_warp + x) * kMostTop + lane] : Top{-INFINITY, 0x7fffffff};
+      const Top other = lane < a.k ? shared.lists[(first_warp + x) * kMostTop + lane] : Top{-INFINITY, 0x7fffffff};
       offer(list, a.k, other.v, other.i, kv, ki);
     }
     if (lane < a.k) put(lane, list);
