@@ -248,28 +248,31 @@ __global__ void __launch_bounds__(kDerivThreads) k_gated_deriv(const GatedDeriv 
   }
 }
 
-// The blocks' sums, in order: 32 values a block, eight threads a value.
-__global__ void __launch_bounds__(256) k_gated_biases(const float* part, int blocks, float* dbg, float* dbu, int h) {
-  __shared__ float red[8][33];
-  grid_dependents_launch();
-  grid_dependency_wait();
+// The blocks' sums, in order: 32 values a block, four threads a value.
+__device__ __forceinline__ void sum_biases(const BiasSums& a, int block) {
+  __shared__ float red[kDerivThreads / 32][33];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const long v = (long)blockIdx.x * 32 + lane;
+  const long v = (long)block * 32 + lane;
   float s = 0.0f;
-  if (v < 2L * h) {
+  if (v < 2L * a.H) {
 #pragma unroll 8
-    for (int b = wid; b < blocks; b += 8) s += part[2L * b * h + v];
+    for (int b = wid; b < a.blocks; b += kDerivThreads / 32) s += a.part[2L * b * a.H + v];
   }
   red[wid][lane] = s;
   __syncthreads();
-  if (wid || v >= 2L * h) return;
+  if (wid || v >= 2L * a.H) return;
 #pragma unroll
-  for (int k = 1; k < 8; k++) s += red[k][lane];
-  if (v < h) {
-    if (dbg) dbg[v] = s;
-  } else if (dbu) {
-    dbu[v - h] = s;
+  for (int k = 1; k < kDerivThreads / 32; k++) s += red[k][lane];
+  if (v < a.H) {
+    if (a.gate) a.gate[v] = s;
+  } else if (a.up) {
+    a.up[v - a.H] = s;
   }
+}
+__global__ void __launch_bounds__(kDerivThreads) k_gated_biases(const BiasSums a) {
+  grid_dependents_launch();
+  grid_dependency_wait();
+  sum_biases(a, blockIdx.x);
 }
 
 __device__ __forceinline__ float power_of(uint32_t max_bits, float* inv) {
@@ -282,6 +285,10 @@ template <int kVec>
 __global__ void __launch_bounds__(kDerivThreads) k_gradient_planes(const GradientPlanes a) {
   grid_dependents_launch();
   grid_dependency_wait();
+  if ((int)blockIdx.x >= a.grid) {           // the biases' sums ride along
+    sum_biases(a.biases, blockIdx.x - a.grid);
+    return;
+  }
   const int blocks_u = (a.H + kDerivThreads * kVec - 1) / (kDerivThreads * kVec), ub = blockIdx.x % blocks_u, cb = blockIdx.x / blocks_u;
   const int r = (ub * kDerivThreads + threadIdx.x) * kVec, lda = aux_rows(a.H);
   if (r >= a.H) return;
@@ -377,12 +384,15 @@ int gated_deriv(const GatedDeriv& d) {
 #undef DERIV
   return check_launch();
 }
-int gradient_planes(const GradientPlanes& g) {
+int gradient_planes(const GradientPlanes& planes) {
+  GradientPlanes g = planes;
   const bool vec = g.H % 4 == 0 && on16(g.gate) && on16(g.up);
   const long blocks = deriv_grid(g.H, g.N, g.cases, vec);
-  if (blocks > 0x7fffffffL) return ERROR_UNSUPPORTED;
-  if (vec) (void)launch_dependent(k_gradient_planes<4>, dim3((unsigned)blocks), dim3(kDerivThreads), 0, stream(), g);
-  else (void)launch_dependent(k_gradient_planes<1>, dim3((unsigned)blocks), dim3(kDerivThreads), 0, stream(), g);
+  const long extra = g.biases.part ? (2L * g.H + 31) / 32 : 0;
+  if (blocks + extra > 0x7fffffffL) return ERROR_UNSUPPORTED;
+  g.grid = (int)blocks;
+  if (vec) (void)launch_dependent(k_gradient_planes<4>, dim3((unsigned)(blocks + extra)), dim3(kDerivThreads), 0, stream(), g);
+  else (void)launch_dependent(k_gradient_planes<1>, dim3((unsigned)(blocks + extra)), dim3(kDerivThreads), 0, stream(), g);
   return check_launch();
 }
 }  // namespace b200
@@ -551,9 +561,10 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     if ((err = split_columns(jobs, split_w ? 3 : 1, V, d.token_max, (int)((after_max - at_tmax) / 4)))) return err;
   }
   if ((err = gated_deriv(d))) return err;
-  if (biases) {
-    (void)launch_dependent(k_gated_biases, dim3((2 * (unsigned)H + 31) / 32), dim3(256), 0, stream(), d.part, blocks,
-                           grad_gate_bias ? grad_gate_bias->data_device : nullptr, grad_up_bias ? grad_up_bias->data_device : nullptr, H);
+  const BiasSums sums = {d.part, blocks, H, grad_gate_bias ? grad_gate_bias->data_device : nullptr,
+                         grad_up_bias ? grad_up_bias->data_device : nullptr};
+  if (biases && !tc) {
+    (void)launch_dependent(k_gated_biases, dim3((2 * (unsigned)H + 31) / 32), dim3(kDerivThreads), 0, stream(), sums);
     if ((err = check_launch())) return err;
   }
   if (!tc) {
@@ -569,6 +580,7 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     return 0;
   }
   GradientPlanes g = {};
+  if (biases) g.biases = sums;
   g.cases = cases;
   g.gate = d.gate;
   g.up = d.up;
@@ -589,35 +601,35 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     g.by_unit[1] = (uint16_t*)(p + at_uu);
   }
   if ((err = gradient_planes(g))) return err;
+  PlaneProduct f[2] = {};
+  int products = 0;
   if (grad_mat) {
-    PlaneProduct f = {};
-    f.npairs = 2;
-    f.a[0] = wgp;
-    f.a[1] = wup;
-    f.b[0] = {g.by_case[0], H, N};
-    f.b[1] = {g.by_case[1], H, N};
-    f.nout = 1;
-    f.out[0] = grad_mat->data_device;
-    f.inv[0] = g.case_inv;
-    f.inv_stride = 1;
-    if ((err = plane_product(f))) return err;
+    PlaneProduct& x = f[products++];
+    x.npairs = 2;
+    x.a[0] = wgp;
+    x.a[1] = wup;
+    x.b[0] = {g.by_case[0], H, N};
+    x.b[1] = {g.by_case[1], H, N};
+    x.nout = 1;
+    x.out[0] = grad_mat->data_device;
+    x.inv[0] = g.case_inv;
+    x.inv_stride = 1;
   }
   if (weights) {
-    PlaneProduct f = {};
-    f.npairs = 1;
-    f.trans = true;
-    f.a[0] = xp;
-    f.inv_stride = 2;
+    PlaneProduct& w = f[products++];
+    w.npairs = 1;
+    w.trans = true;
+    w.a[0] = xp;
+    w.inv_stride = 2;
     cudamat* const out[2] = {grad_gate_w, grad_up_w};
     for (int k = 0; k < 2; k++) {
       if (!out[k]) continue;
-      f.b[f.nout] = {g.by_unit[k], H, N};
-      f.out[f.nout] = out[k]->data_device;
-      f.inv[f.nout++] = g.unit_inv + k;
+      w.b[w.nout] = {g.by_unit[k], H, N};
+      w.out[w.nout] = out[k]->data_device;
+      w.inv[w.nout++] = g.unit_inv + k;
     }
-    if ((err = plane_product(f))) return err;
   }
-  return 0;
+  return plane_products(f, products);
 }
 
 }  // extern "C"

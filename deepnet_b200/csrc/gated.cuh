@@ -66,7 +66,7 @@ struct PlaneProduct {
   const float* inv[2];      // of out's columns; stride inv_stride
   int inv_stride;
 };
-int plane_product(const PlaneProduct& f);
+int plane_products(const PlaneProduct* f, int nproducts);      // one or two, in one launch
 
 // gate, up = their gradients dG, dU from dy; with `maxima` the largest |dG| w_inv, |dU| w_inv of each case (token_max) and the largest
 // |dG| x_inv, |dU| x_inv of each unit (unit_max, gate's and up's): bits of floats, all zero before.  part: sums of dG and dU over the
@@ -82,6 +82,12 @@ struct GatedDeriv {
 };
 int gated_deriv_cases(int H, int N);
 int gated_deriv(const GatedDeriv& d);
+// Sums over the blocks of `part` (GatedDeriv): of dG and dU over all cases.
+struct BiasSums {
+  const float* part;
+  int blocks, H;
+  float *gate, *up;
+};
 // dG and dU as planes: with the weights' scales divided out and one of their own a case (by_case: gate's, up's; inverses case_inv),
 // and with the inputs' scales divided out and one of their own a unit (by_unit; unit_inv 2 x H).  Either may be null.
 struct GradientPlanes {
@@ -91,7 +97,8 @@ struct GradientPlanes {
   const uint32_t *token_max, *unit_max;
   uint16_t *by_case[2], *by_unit[2];
   float *case_inv, *unit_inv;
-  int cases;
+  int cases, grid;          // grid: set by the call
+  BiasSums biases;          // part not null: summed by the same launch
 };
 int gradient_planes(const GradientPlanes& g);
 

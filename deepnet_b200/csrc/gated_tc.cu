@@ -353,33 +353,61 @@ int launch_pairs(void (*kernel)(Params), const Params& p, long tiles) {
 // One operand's K is its columns, so its tiles arrive with M or N contiguous (boxes of 64 x 64) and tcgen05 reads them so; the
 // scales that lie along K are divided out of the other operand when its planes are written.  Tiles of 256 rows by BN columns a
 // pair of CTAs; the rest as above.
-struct ProductParams {
-  CUtensorMap maps[8];                       // a0 hi, lo, a1 hi, lo, b0 hi, lo, b1 hi, lo
-  int M, N, tiles_m, tiles_n, npairs, nout, k_iters, inv_stride;
-  int splits;                                // > 1: each tile's stages are shared out; split s leaves its sums in part + s * M * N
+// Two products share a launch, so that few tiles of either leave fewer SMs without work.
+struct ProductPart {
+  int M, N, tiles_m, tiles_n, npairs, nout, trans, k_iters, inv_stride;
+  int a_map, b_map;                          // first of its tensor maps: a0 hi, lo, (a1 hi, lo); b0 hi, lo, (b1 hi, lo)
+  int splits;                                // > 1: each tile's stages are shared out; split s leaves its sums in part + s * nout * M * N
+  int items;                                 // tiles times splits
   float* part;
   float* out[2];
   const float* inv[2];
+};
+struct ProductParams {
+  CUtensorMap maps[14];
+  ProductPart product[2];
+  int nmaps, items;
   int* status;
   uint32_t spin_limit, stage_tx;
+};
+// Where item w belongs.
+struct ProductItem {
+  int which, out, tm, tn, split, first, last;     // first, last: stages
+  __device__ __forceinline__ ProductItem(const ProductParams& p, int w) {
+    which = w >= p.product[0].items;
+    const ProductPart& q = p.product[which];
+    w -= which ? p.product[0].items : 0;
+    split = w % q.splits;
+    tile_coords_g<8>(w / q.splits, q.tiles_m, q.tiles_n * q.nout, tm, tn);
+    out = tn >= q.tiles_n;
+    tn -= out * q.tiles_n;
+    const long all = (long)q.k_iters * q.npairs;
+    first = (int)(all * split / q.splits);
+    last = (int)(all * (split + 1) / q.splits);
+  }
 };
 
 // The splits' sums in order, times the columns' scales.
 __global__ void __launch_bounds__(256) k_plane_finish(const __grid_constant__ ProductParams p) {
   grid_dependents_launch();
   grid_dependency_wait();
-  const long n = (long)p.M * p.N, all = n * p.nout;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long)gridDim.x * blockDim.x) {
-    float s = 0.0f;
+#pragma unroll 1
+  for (int which = 0; which < 2; which++) {
+    const ProductPart& q = p.product[which];
+    if (q.items == 0 || q.splits == 1) continue;
+    const long n = (long)q.M * q.N, all = n * q.nout;
+    for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long)gridDim.x * blockDim.x) {
+      float s = 0.0f;
 #pragma unroll 8
-    for (int k = 0; k < p.splits; k++) s += p.part[all * k + i];
-    const int o = i >= n;
-    const long at = i - o * n;
-    p.out[o][at] = s * p.inv[o][at / p.M * p.inv_stride];
+      for (int k = 0; k < q.splits; k++) s += q.part[all * k + i];
+      const int o = i >= n;
+      const long at = i - o * n;
+      q.out[o][at] = s * q.inv[o][at / q.M * q.inv_stride];
+    }
   }
 }
 
-template <int BN, bool kTrans>
+template <int BN>
 __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_constant__ ProductParams p) {
   using T = Tile<BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -394,10 +422,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const uint32_t limit = p.spin_limit;
-  const int tiles_n = p.tiles_n * p.nout, splits = p.splits, items = p.tiles_m * tiles_n * splits, first = blockIdx.x >> 1, step = gridDim.x >> 1;
-  const int all_iters = p.k_iters * p.npairs;
-  auto of_split = [&](int s) { return (int)((long)all_iters * s / splits); };     // its first stage
-  if (warp == 2 && lane < 8) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.maps[lane]) : "memory");
+  const int items = p.items, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  if (warp == 2 && lane < p.nmaps) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.maps[lane]) : "memory");
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < kStages; s++) {
@@ -431,7 +457,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
     if (warp == 0) {
       // copies: lanes 0-3 a plane of 64 of this CTA's 128 rows, lanes 4 on a plane of its half of the columns (64 at a time where
       // they are contiguous)
-      constexpr int kBoxes = kTrans ? BN / 128 : 1;
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -439,14 +464,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
       const int plane = lane & 1, box = is_a ? lane >> 1 : (lane - 4) >> 1;
       const uint32_t to = is_a ? plane * 16384u + box * 8192u : 32768u + plane * (uint32_t)(BN * 64) + box * 8192u;
       for (int w = first; w < items && ok; w += step) {
-        int tm, tn;
-        tile_coords_g<8>(w / splits, p.tiles_m, tiles_n, tm, tn);
-        const int o = tn >= p.tiles_n, n0 = (tn - o * p.tiles_n) * BN + (int)rank * (BN / 2);
-        const int row = is_a ? tm * 256 + (int)rank * 128 + 64 * box : n0 + 64 * box;
-        const int last = of_split(w % splits + 1);
-        int it = of_split(w % splits), q = it / p.k_iters, kb = it - q * p.k_iters;
-        for (; it < last; it++) {
-          const CUtensorMap* map = &p.maps[(is_a ? 2 * q : 4 + 2 * (kTrans ? o : q)) + plane];
+        const ProductItem at(p, w);
+        const ProductPart& part = p.product[at.which];
+        const int row = (is_a ? at.tm * 256 + (int)rank * 128 : at.tn * BN + (int)rank * (BN / 2)) + 64 * box;
+        const int per = part.k_iters, trans = part.trans;
+        const bool mine = is_a || lane < 4 + (trans ? 2 * (BN / 128) : 2);
+        int q = at.first / per, kb = at.first - q * per;
+        for (int it = at.first; it < at.last; it++) {
+          const CUtensorMap* map = &p.maps[(is_a ? part.a_map + 2 * q : part.b_map + 2 * (trans ? at.out : q)) + plane];
           if (!mbar_wait(empty(stage), phase ^ 1u, &abort_flag, limit)) {
             gave_up(35);
             ok = false;
@@ -454,13 +479,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
           }
           const uint32_t bar = full(stage), dst = base + stage * T::kStageBytes + to;
           if (lane == 0 && rank == 0) mbar_expect_tx(bar, p.stage_tx);
-          if (is_a || (kTrans && lane < 4 + 2 * kBoxes)) tma_load_2d_pair(dst, map, row, kb * kK, bar);
-          else if (!kTrans && lane < 6) tma_load_2d_pair(dst, map, kb * kK, row, bar);
+          if (mine) {
+            const bool along = is_a || trans;            // rows are the contiguous dimension
+            tma_load_2d_pair(dst, map, along ? row : kb * kK, along ? kb * kK : row, bar);
+          }
           if (++stage == T::kNumStages) {
             stage = 0;
             phase ^= 1u;
           }
-          if (++kb == p.k_iters) {
+          if (++kb == per) {
             kb = 0;
             q++;
           }
@@ -470,16 +497,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
         for (int i = 0; i < 1024; i++) __nanosleep(100);
     } else if (warp == 1 && rank == 0) {
       const bool elected = elect_one();
-      const uint32_t idesc = (1u << 4) | (1u << 15) | ((kTrans ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((256u >> 4) << 24);
       // M or N contiguous: blocks of 64 (a row of 128 bytes an element of K) 64 rows apart; sixteen rows a step.  K-major as above.
       constexpr uint32_t kMn = ((uint32_t)(kK * 128) >> 4) << 16, kStepMn = 2048u >> 4;
-      constexpr uint32_t kB = kTrans ? kMn : 1u << 16, kStepB = kTrans ? kStepMn : 2u;
       int stage = 0;
       uint32_t phase = 0, chunk = 0;
       bool ok = true;
       for (int w = first; w < items && ok; w += step) {
         int in_chunk = 0;
-        const int iters = of_split(w % splits + 1) - of_split(w % splits);
+        const ProductItem at(p, w);
+        const int iters = at.last - at.first;
+        const uint32_t trans = (uint32_t)p.product[at.which].trans;
+        const uint32_t idesc = (1u << 4) | (1u << 15) | (trans << 16) | ((uint32_t)(BN >> 3) << 17) | ((256u >> 4) << 24);
+        const uint32_t b_lead = trans ? kMn : 1u << 16, b_step = trans ? kStepMn : 2u;
         for (int kb = 0; kb < iters; kb++) {
           const int acc = chunk & 1;
           if (in_chunk == 0) {
@@ -503,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
 #pragma unroll
             for (int j = 0; j < kK / 16; j++) {
               const uint64_t da = ((uint64_t)kDescK << 32) | (uint64_t)(kMn + a + kStepMn * j);
-              const uint64_t db = ((uint64_t)kDescK << 32) | (uint64_t)(kB + b + kStepB * j);
+              const uint64_t db = ((uint64_t)kDescK << 32) | (uint64_t)(b_lead + b + b_step * j);
               if (elected) mma_f16_pair(tmem + acc * BN, da, db, idesc, i + j > 0 || in_chunk > 0);
             }
           }
@@ -527,11 +556,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
     uint32_t chunk = 0;
     bool ok = true;
     for (int w = first; w < items && ok; w += step) {
-      int tm, tn;
-      tile_coords_g<8>(w / splits, p.tiles_m, tiles_n, tm, tn);
-      const int o = tn >= p.tiles_n, n0 = (tn - o * p.tiles_n) * BN + half * kCols;
-      const int m = tm * 256 + (int)rank * 128 + q * 32 + lane;
-      const int sp = w % splits, chunks = (of_split(sp + 1) - of_split(sp) + kChunk - 1) / kChunk;
+      const ProductItem at(p, w);
+      const ProductPart& part = p.product[at.which];
+      const int o = at.out, n0 = at.tn * BN + half * kCols, m = at.tm * 256 + (int)rank * 128 + q * 32 + lane;
+      const int chunks = (at.last - at.first + kChunk - 1) / kChunk;
       float sum[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; j++) sum[j] = 0.0f;
@@ -558,19 +586,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
         if (lane == 0) mbar_arrive_leader(free_(acc), 0);
       }
       if (!ok) break;
-      const int live = m < p.M ? p.N - n0 : 0;
-      if (splits > 1) {
-        float* part = p.part + ((long)sp * p.nout + o) * p.M * p.N + (long)n0 * p.M + m;
+      const long M = part.M;
+      const int live = m < part.M ? part.N - n0 : 0;
+      if (part.splits > 1) {
+        float* to = part.part + ((long)at.split * part.nout + o) * M * part.N + n0 * M + m;
 #pragma unroll
         for (int j = 0; j < kCols; j++)
-          if (j < live) part[(long)j * p.M] = sum[j];
+          if (j < live) to[j * M] = sum[j];
         continue;
       }
-      const float* inv = p.inv[o] + (long)n0 * p.inv_stride;
-      float* out = p.out[o] + (long)n0 * p.M + m;
+      const int stride = part.inv_stride;
+      const float* inv = part.inv[o] + (long)n0 * stride;
+      float* out = part.out[o] + n0 * M + m;
 #pragma unroll
       for (int j = 0; j < kCols; j++)
-        if (j < live) out[(long)j * p.M] = sum[j] * __ldg(inv + (long)j * p.inv_stride);
+        if (j < live) out[j * M] = sum[j] * __ldg(inv + (long)j * stride);
     }
   }
   tc_fence_before();
@@ -768,56 +798,79 @@ int gated_tc(const GatedForward& f) {
   return launch_pairs(k_gated_tc<32>, p, tiles);
 }
 
-int plane_product(const PlaneProduct& f) {
+int plane_products(const PlaneProduct* f, int nproducts) {
   ProductParams p = {};
-  p.M = f.a[0].rows;
-  p.N = f.trans ? f.b[0].rows : f.b[0].cols;
-  p.npairs = f.npairs;
-  p.nout = f.nout;
-  p.k_iters = (f.a[0].cols + kK - 1) / kK;
-  p.inv_stride = f.inv_stride;
-  for (int i = 0; i < f.nout; i++) {
-    p.out[i] = f.out[i];
-    p.inv[i] = f.inv[i];
-  }
   p.status = status_word();
   p.spin_limit = wait_limit();
-  p.tiles_m = (p.M + 255) / 256;
-  // the wider tile reads less shared memory a multiply-add; the narrower one where it needs fewer turns of the pairs
   const long pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
-  auto turns = [&](int w) { return ((long)p.tiles_m * f.nout * ((p.N + w - 1) / w) + pairs - 1) / pairs; };
-  const int bn = 2 * turns(256) <= turns(128) * 1.1 ? 256 : 128;
-  p.tiles_n = (p.N + bn - 1) / bn;
-  // too few tiles for the device and long sums: each tile's stages are shared out, eight or more to a pair
-  const int all_iters = p.k_iters * f.npairs;
-  long splits = pairs / ((long)p.tiles_m * p.tiles_n * f.nout);
-  if (splits > all_iters / 8) splits = all_iters / 8;
-  p.splits = splits < 1 ? 1 : (int)splits;
-  CallScratch room(2, p.splits > 1 ? (size_t)p.splits * f.nout * p.M * p.N * sizeof(float) : 0);
-  p.part = (float*)room.p;
-  if (p.splits > 1 && !p.part) return CUDA_ERROR;
-  const long tiles = (long)p.tiles_m * p.tiles_n * f.nout * p.splits;
-  if (tiles > 0x7fffffffL) return ERROR_UNSUPPORTED;
-  const int nb = f.trans ? f.nout : f.npairs;
-  for (int i = 0; i < 8; i++) {
-    const int which = (i >> 1) & 1;
-    const bool is_a = i < 4;
-    if (which >= (is_a ? f.npairs : nb)) {
-      p.maps[i] = p.maps[i - 2];
-      continue;
+  // The wider tile reads less shared memory a multiply-add; the narrower one where it needs fewer turns of the pairs.  Work counted in
+  // stages of a tile.
+  auto stages = [&](int w) {
+    long n = 0;
+    for (int i = 0; i < nproducts; i++) {
+      const long N = f[i].trans ? f[i].b[0].rows : f[i].b[0].cols;
+      n += (long)((f[i].a[0].rows + 255) / 256) * f[i].nout * ((N + w - 1) / w) * f[i].npairs * ((f[i].a[0].cols + kK - 1) / kK);
     }
-    const Planes& m = is_a ? f.a[which] : f.b[which];
-    const int lda = aux_rows(m.rows);
-    if (!plane_map(&p.maps[i], m.p + ((i & 1) ? 0 : lda), (uint64_t)m.rows, (uint64_t)m.cols, 2 * (uint64_t)lda, kK,
-                   is_a || f.trans ? kK : bn / 2))
-      return set_error("cuTensorMapEncodeTiled failed for a plane");
+    return n;
+  };
+  const int bn = 2 * ((stages(256) + pairs - 1) / pairs) <= 1.1 * ((stages(128) + pairs - 1) / pairs) ? 256 : 128;
+  const long share = (stages(bn) + pairs - 1) / pairs;       // stages a pair has to do at least
+  size_t bytes = 0;
+  long items = 0;
+  for (int i = 0; i < nproducts; i++) {
+    ProductPart& q = p.product[i];
+    q.M = f[i].a[0].rows;
+    q.N = f[i].trans ? f[i].b[0].rows : f[i].b[0].cols;
+    q.npairs = f[i].npairs;
+    q.nout = f[i].nout;
+    q.trans = f[i].trans;
+    q.k_iters = (f[i].a[0].cols + kK - 1) / kK;
+    q.inv_stride = f[i].inv_stride;
+    q.tiles_m = (q.M + 255) / 256;
+    q.tiles_n = (q.N + bn - 1) / bn;
+    // a sum that is longer than a pair's share is shared out, eight stages or more to a pair
+    const long all = (long)q.k_iters * q.npairs, least = share > 8 ? share : 8;
+    long splits = (all + least / 2) / least;
+    if (splits > 64) splits = 64;
+    q.splits = splits < 1 ? 1 : (int)splits;
+    const long n = (long)q.tiles_m * q.tiles_n * q.nout * q.splits;
+    items += n;
+    if (items > 0x3fffffffL) return ERROR_UNSUPPORTED;
+    q.items = (int)n;
+    if (q.splits > 1) bytes += (size_t)q.splits * q.nout * q.M * q.N * sizeof(float);
+    q.a_map = p.nmaps;
+    for (int side = 0; side < 2; side++) {
+      const int count = side == 0 ? q.npairs : f[i].trans ? q.nout : q.npairs;
+      if (side) q.b_map = p.nmaps;
+      for (int m = 0; m < 2 * count; m++) {
+        const Planes& x = side ? f[i].b[m >> 1] : f[i].a[m >> 1];
+        const int lda = aux_rows(x.rows);
+        if (!plane_map(&p.maps[p.nmaps++], x.p + ((m & 1) ? 0 : lda), (uint64_t)x.rows, (uint64_t)x.cols, 2 * (uint64_t)lda, kK,
+                       side == 0 || f[i].trans ? kK : bn / 2))
+          return set_error("cuTensorMapEncodeTiled failed for a plane");
+      }
+    }
+    for (int o = 0; o < q.nout; o++) {
+      q.out[o] = f[i].out[o];
+      q.inv[o] = f[i].inv[o];
+    }
+  }
+  p.items = (int)items;
+  CallScratch room(2, bytes);
+  if (bytes && !room.p) return CUDA_ERROR;
+  float* at = (float*)room.p;
+  long finished = 0;
+  for (int i = 0; i < nproducts; i++) {
+    ProductPart& q = p.product[i];
+    if (q.splits == 1) continue;
+    q.part = at;
+    at += (size_t)q.splits * q.nout * q.M * q.N;
+    finished += (long)q.nout * q.M * q.N;
   }
   p.stage_tx = 2 * (32 * 1024 + bn * 128) + (uint32_t)take_injected_bytes();
-  int err;
-  if (f.trans) err = bn == 256 ? launch_pairs(k_plane_product<256, true>, p, tiles) : launch_pairs(k_plane_product<128, true>, p, tiles);
-  else err = bn == 256 ? launch_pairs(k_plane_product<256, false>, p, tiles) : launch_pairs(k_plane_product<128, false>, p, tiles);
-  if (err || p.splits == 1) return err;
-  long blocks = ((long)p.M * p.N * f.nout + 255) / 256;
+  const int err = bn == 256 ? launch_pairs(k_plane_product<256>, p, items) : launch_pairs(k_plane_product<128>, p, items);
+  if (err || !bytes) return err;
+  long blocks = (finished + 255) / 256;
   if (blocks > 8L * sm_count()) blocks = 8L * sm_count();
   (void)launch_dependent(k_plane_finish, dim3((unsigned)blocks), dim3(256), 0, stream(), p);
   return check_launch();
