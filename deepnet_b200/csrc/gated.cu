@@ -518,7 +518,7 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
   const bool aligned = V % 4 == 0 && H % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device) &&
                        on16(gate->data_device) && on16(up->data_device);
   const bool few = aligned && !gate_planes && N < 256 && (long)V * H >= 1L << 22;
-  const bool large = (long)V * H * N >= 1L << (aligned ? 26 : 22) && !few;
+  const bool large = (long)V * H * N >= 1L << 16 && !few;
   const bool tc = V > 0 && (weights || grad_mat) && gemm_path() != 2 && (large || gemm_path() == 1) && tma_available();
   const int cases = gated_deriv_cases(H, N), blocks = (N + cases - 1) / cases;
   const bool split_w = tc && !gate_planes;

@@ -27,7 +27,7 @@ namespace {
 constexpr int kK = 64;                       // products of a stage: 128 bytes of a plane
 constexpr int kRing = 192 * 1024;
 constexpr int kExchange = 32 * 1024;         // two buffers of 16 columns each way for four pairs of warps
-constexpr int kSmem = kRing + kExchange + 1024 /*alignment*/ + 256 /*barriers*/;
+constexpr int kSmem = kRing + kExchange + 1024 /*alignment*/ + 1024 /*scales*/ + 256 /*barriers*/;
 constexpr int kThreads = 384, kEpiThreads = 256;
 constexpr int kStages = 6;                   // most of any tile width
 constexpr int kChunk = 128 / kK;             // stages an accumulator sums
@@ -77,16 +77,23 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
       : "memory");
 }
 
-// Whether `ok` holds in all of 64 threads, which wait for each other at barrier `id`.
-__device__ __forceinline__ bool all_ok(int id, bool ok) {
+// Whether two scales multiply to a normal number.
+__device__ __forceinline__ bool tame(float scale) { return scale >= 8.6736174e-19f && scale <= 1.1529215e18f; }      // 2^-60, 2^60
+__device__ __forceinline__ float4 lds_f4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+  return v;
+}
+// Whether `ok` holds in all of `threads` threads, which wait for each other at barrier `id`.
+__device__ __forceinline__ bool all_ok(int id, int threads, bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %2, 0;\n\t"
-      "bar.red.and.pred p, %1, 64, q;\n\t"
+      "setp.ne.u32 q, %3, 0;\n\t"
+      "bar.red.and.pred p, %1, %2, q;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(r)
-      : "r"(id), "r"((uint32_t)ok)
+      : "r"(id), "r"(threads), "r"((uint32_t)ok)
       : "memory");
   return r != 0;
 }
@@ -103,7 +110,7 @@ template <int BN>
 __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant__ GatedParams p) {
   using T = Tile<BN>;
   extern __shared__ uint8_t smem_raw[];
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, exchange = base + kRing, bars = exchange + kExchange;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, exchange = base + kRing, scales = exchange + kExchange, bars = scales + 1024;
   auto full = [&](int s) { return bars + 8u * s; };                 // the stage's copies, of both CTAs, in the leader
   auto empty = [&](int s) { return bars + 8u * (kStages + s); };    // the stage has been multiplied
   auto done = [&](int a) { return bars + 8u * (2 * kStages + a); }; // the accumulator holds its chunk
@@ -240,10 +247,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
       int tm, tn;
       tile_coords_g<8>(t, p.tiles_m, p.tiles_n, tm, tn);
       const int unit = tm * 128 + (int)rank * 64 + (q & 1) * 32 + lane, n0 = tn * BN + half * kCols;
+      // (asked for here, wanted behind the sums)
+      const float2 r = unit < p.M ? make_float2(p.w_inv[2L * unit], p.w_inv[2L * unit + 1]) : make_float2(1.0f, 1.0f);
+      const float bg = unit < p.M && p.bg ? p.bg[unit] : 0.0f, bu = unit < p.M && p.bu ? p.bu[unit] : 0.0f;
+      const int case_of_mine = tn * BN + (int)threadIdx.x - 128;
+      const float c = (int)threadIdx.x - 128 < BN && case_of_mine < p.N ? p.x_inv[case_of_mine] : 1.0f;
       float sum[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; j++) sum[j] = 0.0f;
-      for (int c = 0; c < chunks; c++, chunk++) {
+      for (int k = 0; k < chunks; k++, chunk++) {
         const int acc = chunk & 1;
         if (!mbar_wait(done(acc), (chunk >> 1) & 1u, &abort_flag, limit)) {
           gave_up(34);
@@ -265,20 +277,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
         __syncwarp();
         if (lane == 0) mbar_arrive_leader(free_(acc), 0);
       }
-      // both warps of a pair go on, or neither: they wait for each other below
-      ok = all_ok(1 + pair, ok);
-      if (!ok) break;
+      // All drain warps go on, or none: they wait for each other here and below.  The cases' scales are there for all of them; where no
+      // product of two scales leaves the range of normal numbers, one multiplication takes both.
       const bool in = unit < p.M;
-      const float2 r = in ? make_float2(p.w_inv[2L * unit], p.w_inv[2L * unit + 1]) : make_float2(0.0f, 0.0f);
-      const float bg = in && p.bg ? p.bg[unit] : 0.0f, bu = in && p.bu ? p.bu[unit] : 0.0f;
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + (threadIdx.x - 128) * 4u), "f"(c) : "memory");
+      ok = all_ok(5, kEpiThreads, ok);
+      if (!ok) break;
+      const bool plain = all_ok(5, kEpiThreads, tame(c) && tame(r.x) && tame(r.y));
       float *yo = p.y + unit, *go = p.gate + unit, *uo = p.up + unit;
 #pragma unroll 1
       for (int round = 0; round < kCols / 16; round++) {
         const uint32_t buf = stage_at + (uint32_t)(round & 1) * 4096u;
-        float c[8];
         const int first_n = n0 + 16 * round + 8 * which;
-#pragma unroll
-        for (int i = 0; i < 8; i++) c[i] = first_n + i < p.N ? __ldg(p.x_inv + first_n + i) : 1.0f;
 #pragma unroll
         for (int x = 0; x < kCols / 16; x++)
           if (x == round) {
@@ -287,16 +297,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
               asm volatile("st.shared.f32 [%0], %1;" ::"r"(buf + (uint32_t)which * 2048u + i * 128), "f"(sum[16 * x + i]));
           }
         named_bar_sync(1 + pair, 64);
-        float gs[8], us[8];
+        float gs[8], us[8], c8[8];
+        const uint32_t scale_at = scales + (uint32_t)(half * kCols + 16 * round + 8 * which) * 4u;
+        const float4 c0 = lds_f4(scale_at), c1 = lds_f4(scale_at + 16);
+        c8[0] = c0.x; c8[1] = c0.y; c8[2] = c0.z; c8[3] = c0.w; c8[4] = c1.x; c8[5] = c1.y; c8[6] = c1.z; c8[7] = c1.w;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           asm volatile("ld.shared.f32 %0, [%1];" : "=f"(gs[i]) : "r"(buf + (uint32_t)(8 * which + i) * 128u));
           asm volatile("ld.shared.f32 %0, [%1];" : "=f"(us[i]) : "r"(buf + 2048u + (uint32_t)(8 * which + i) * 128u));
         }
+        if (plain) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          gs[i] = unscale(gs[i], r.x, c[i]) + bg;
-          us[i] = unscale(us[i], r.y, c[i]) + bu;
+          for (int i = 0; i < 8; i++) {
+            gs[i] = fmaf(gs[i], r.x * c8[i], bg);
+            us[i] = fmaf(us[i], r.y * c8[i], bu);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            gs[i] = unscale(gs[i], r.x, c8[i]) + bg;
+            us[i] = unscale(us[i], r.y, c8[i]) + bu;
+          }
         }
         const int live = in ? min(8, p.N - first_n) : 0;
         if (p.gate) {
