@@ -280,9 +280,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
       // All drain warps go on, or none: they wait for each other here and below.  The cases' scales are there for all of them; where no
       // product of two scales leaves the range of normal numbers, one multiplication takes both.
       const bool in = unit < p.M;
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + (threadIdx.x - 128) * 4u), "f"(c) : "memory");
       ok = all_ok(5, kEpiThreads, ok);
       if (!ok) break;
+      // (everybody is done with the last tile's)
+      if ((int)threadIdx.x - 128 < BN) asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + (threadIdx.x - 128) * 4u), "f"(c) : "memory");
       const bool plain = all_ok(5, kEpiThreads, tame(c) && tame(r.x) && tame(r.y));
       float *yo = p.y + unit, *go = p.gate + unit, *uo = p.up + unit;
 #pragma unroll 1
