@@ -80,7 +80,7 @@ struct GatedDeriv {
   float* part;
   int cases;                // of a block
 };
-int gated_deriv_cases(int H, int N);
+int gated_deriv_cases(int N);
 int gated_deriv(const GatedDeriv& d);
 // Sums over the blocks of `part` (GatedDeriv): of dG and dU over all cases.
 struct BiasSums {
@@ -97,7 +97,7 @@ struct GradientPlanes {
   const uint32_t *token_max, *unit_max;
   uint16_t *by_case[2], *by_unit[2];
   float *case_inv, *unit_inv;
-  int cases, grid;          // grid: set by the call
+  int cases, grid;          // set by the call
   BiasSums biases;          // part not null: summed by the same launch
 };
 int gradient_planes(const GradientPlanes& g);

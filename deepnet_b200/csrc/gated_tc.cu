@@ -37,6 +37,8 @@ constexpr uint32_t kDescK = (1024u >> 4) | (1u << 14) | (2u << 29);   // K-major
 struct GatedParams {
   CUtensorMap maps[6];                       // gate hi, lo, up hi, lo, x hi, lo
   int M, N, K, tiles_m, tiles_n, activation;
+  int splits;                                // > 1: each tile's stages are shared out; split s leaves its sums in part + s * 2 * M * N
+  float* part;                               // (gate's, then up's)
   const float *w_inv, *x_inv, *bg, *bu;
   float *gate, *up, *y;
   int* status;
@@ -121,8 +123,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const uint32_t limit = p.spin_limit;
-  const int tiles = p.tiles_m * p.tiles_n, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int splits = p.splits, items = p.tiles_m * p.tiles_n * splits, first = blockIdx.x >> 1, step = gridDim.x >> 1;
   const int k_iters = (p.K + kK - 1) / kK;
+  auto of_split = [&](int s) { return (int)((long)k_iters * s / splits); };       // its first stage
   if (warp == 2 && lane < 6) asm volatile("prefetch.tensormap [%0];" ::"l"(&p.maps[lane]) : "memory");
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -161,11 +164,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
       bool ok = true;
       const bool is_a = lane < 4;
       const uint32_t to = is_a ? (lane & 1) * 16384u + (lane >> 1) * 8192u : 32768u + (lane & 1) * (uint32_t)(BN * 64);
-      for (int t = first; t < tiles && ok; t += step) {
+      for (int w = first; w < items && ok; w += step) {
         int tm, tn;
-        tile_coords_g<8>(t, p.tiles_m, p.tiles_n, tm, tn);
+        tile_coords_g<8>(w / splits, p.tiles_m, p.tiles_n, tm, tn);
         const int row = is_a ? tm * 128 + (int)rank * 64 : tn * BN + (int)rank * (BN / 2);
-        for (int kb = 0; kb < k_iters; kb++) {
+        const int last = of_split(w % splits + 1);
+        for (int kb = of_split(w % splits); kb < last; kb++) {
           if (!mbar_wait(empty(stage), phase ^ 1u, &abort_flag, limit)) {
             gave_up(31);
             ok = false;
@@ -190,9 +194,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
       int stage = 0;
       uint32_t phase = 0, chunk = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
+      for (int w = first; w < items && ok; w += step) {
         int in_chunk = 0;
-        for (int kb = 0; kb < k_iters; kb++) {
+        const int last = of_split(w % splits + 1);
+        for (int kb = of_split(w % splits); kb < last; kb++) {
           const int acc = chunk & 1;
           if (in_chunk == 0) {
             if (!mbar_wait(free_(acc), ((chunk >> 1) & 1u) ^ 1u, &abort_flag, limit)) {
@@ -224,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
             stage = 0;
             phase ^= 1u;
           }
-          if (++in_chunk == kChunk || kb == k_iters - 1) {
+          if (++in_chunk == kChunk || kb == last - 1) {
             if (elected) mma_commit_pair(done(acc), 3);
             chunk++;
             in_chunk = 0;
@@ -241,17 +246,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
     const int ew = warp - 4, q = warp & 3, half = ew >> 2, which = q >> 1, pair = (q & 1) * 2 + half;
     const uint32_t stage_at = exchange + (uint32_t)(pair * 8192 + lane * 4);
     uint32_t chunk = 0;
-    const int chunks = (k_iters + kChunk - 1) / kChunk;
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += step) {
+    for (int w = first; w < items && ok; w += step) {
       int tm, tn;
-      tile_coords_g<8>(t, p.tiles_m, p.tiles_n, tm, tn);
+      tile_coords_g<8>(w / splits, p.tiles_m, p.tiles_n, tm, tn);
       const int unit = tm * 128 + (int)rank * 64 + (q & 1) * 32 + lane, n0 = tn * BN + half * kCols;
       // (asked for here, wanted behind the sums)
       const float2 r = unit < p.M ? make_float2(p.w_inv[2L * unit], p.w_inv[2L * unit + 1]) : make_float2(1.0f, 1.0f);
       const float bg = unit < p.M && p.bg ? p.bg[unit] : 0.0f, bu = unit < p.M && p.bu ? p.bu[unit] : 0.0f;
       const int case_of_mine = tn * BN + (int)threadIdx.x - 128;
       const float c = (int)threadIdx.x - 128 < BN && case_of_mine < p.N ? p.x_inv[case_of_mine] : 1.0f;
+      const int sp = w % splits, chunks = (of_split(sp + 1) - of_split(sp) + kChunk - 1) / kChunk;
       float sum[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; j++) sum[j] = 0.0f;
@@ -276,6 +281,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_leader(free_(acc), 0);
+      }
+      if (splits > 1) {
+        if (!ok) break;
+        float* to = p.part + ((long)(sp * 2 + which) * p.N + n0) * p.M + unit;
+        const int live = unit < p.M ? p.N - n0 : 0;
+#pragma unroll
+        for (int j = 0; j < kCols; j++)
+          if (j < live) to[(long)j * p.M] = sum[j];
+        continue;
       }
       // All drain warps go on, or none: they wait for each other here and below.  The cases' scales are there for all of them; where no
       // product of two scales leaves the range of normal numbers, one multiplication takes both.
@@ -342,6 +356,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_gated_tc(const __grid_constant_
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc2(tmem, T::kTmemCols);
+  }
+}
+
+// The splits' sums in order, and what the epilogue does with them.
+template <int kAct>
+__global__ void __launch_bounds__(256) k_gated_finish(const __grid_constant__ GatedParams p) {
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const long all = (long)p.M * p.N;
+  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long)gridDim.x * blockDim.x) {
+    const int n = (int)(i / p.M), unit = (int)(i - (long)n * p.M);
+    float g = 0.0f, u = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < p.splits; k++) {
+      g += p.part[2 * all * k + i];
+      u += p.part[2 * all * k + all + i];
+    }
+    const float c = p.x_inv[n];
+    g = unscale(g, p.w_inv[2L * unit], c) + (p.bg ? p.bg[unit] : 0.0f);
+    u = unscale(u, p.w_inv[2L * unit + 1], c) + (p.bu ? p.bu[unit] : 0.0f);
+    if (p.gate) {
+      p.gate[i] = g;
+      p.up[i] = u;
+    }
+    float slope;
+    p.y[i] = activate<kAct>(g, slope) * u;
   }
 }
 
@@ -582,6 +622,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
       const ProductPart& part = p.product[at.which];
       const int o = at.out, n0 = at.tn * BN + half * kCols, m = at.tm * 256 + (int)rank * 128 + q * 32 + lane;
       const int chunks = (at.last - at.first + kChunk - 1) / kChunk;
+      // the columns' scales, one a lane (asked for here, wanted behind the sums)
+      float scales[(kCols + 31) / 32];
+#pragma unroll
+      for (int g = 0; g < (kCols + 31) / 32; g++) {
+        const int n = n0 + 32 * g + lane;
+        scales[g] = n < part.N ? part.inv[o][(long)n * part.inv_stride] : 0.0f;
+      }
       float sum[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; j++) sum[j] = 0.0f;
@@ -617,12 +664,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_plane_product(const __grid_cons
           if (j < live) to[j * M] = sum[j];
         continue;
       }
-      const int stride = part.inv_stride;
-      const float* inv = part.inv[o] + (long)n0 * stride;
       float* out = part.out[o] + n0 * M + m;
 #pragma unroll
-      for (int j = 0; j < kCols; j++)
-        if (j < live) out[j * M] = sum[j] * __ldg(inv + (long)j * stride);
+      for (int j = 0; j < kCols; j++) {
+        const float c = __shfl_sync(0xffffffffu, scales[j / 32], j % 32);
+        if (j < live) out[j * M] = sum[j] * c;
+      }
     }
   }
   tc_fence_before();
@@ -786,18 +833,25 @@ int gated_tc(const GatedForward& f) {
   p.status = status_word();
   p.spin_limit = wait_limit();
   p.tiles_m = (p.M + 127) / 128;
-  // The tile's width: what the pairs of CTAs need for their share of the tiles, a stage taking as long as its twelve
-  // instructions (half a cycle a column) or, below that, as its copies.
-  const int widths[4] = {256, 128, 64, 32};
+  // The tile's width, and whether the sums are shared out: what the pairs of CTAs need for their share of the work, in cycles.  A
+  // stage takes as long as its instructions (6 BN) or the rows its copies bring (3.6 each: 4096 x 64, 64 cases, a single tile, 0.55
+  // us a stage at any width); sums that are shared out cost a launch and their way through memory.
+  const long pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, stages = (p.K + kK - 1) / kK;
   int bn = 256;
   double best = 0;
-  for (int w : widths) {
-    const long tiles = (long)p.tiles_m * ((p.N + w - 1) / w), pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
-    const double stage = 6.0 * w > 500.0 ? 6.0 * w : 500.0;
-    const double cost = (double)((tiles + pairs - 1) / pairs) * (stage * ((p.K + kK - 1) / kK) + 2000.0 + 8.0 * w);
-    if (w == 256 || cost < 0.98 * best) {
-      best = cost;
-      bn = w;
+  for (int w = 256; w >= 32; w /= 2) {
+    const long tiles = (long)p.tiles_m * ((p.N + w - 1) / w);
+    for (long s = 1; s <= 16 && s * 2 <= (stages > 2 ? stages : 2); s++) {
+      const long turns = (tiles * s + pairs - 1) / pairs;
+      if (s > 1 && turns > 1) break;
+      const double stage = 6.0 * w > 3.6 * (256 + w) ? 6.0 * w : 3.6 * (256 + w);
+      const double cost = turns * (stage * ((stages + s - 1) / s) + 2500.0 + 10.0 * w) +
+                          (s > 1 ? 12000.0 + (double)s * p.M * p.N * 8.0 / 1500.0 : 0.0);
+      if (best == 0 || cost < 0.97 * best) {
+        best = cost;
+        bn = w;
+        p.splits = (int)s;
+      }
     }
   }
   p.tiles_n = (p.N + bn - 1) / bn;
@@ -809,15 +863,26 @@ int gated_tc(const GatedForward& f) {
     if (!plane_map(&p.maps[i], m.p + ((i & 1) ? 0 : lda), (uint64_t)m.rows, (uint64_t)m.cols, 2 * (uint64_t)lda, kK, i < 4 ? 64 : bn / 2))
       return set_error("cuTensorMapEncodeTiled failed for a plane");
   }
-  const long tiles = (long)p.tiles_m * p.tiles_n;
+  const long tiles = (long)p.tiles_m * p.tiles_n * p.splits;
   if (tiles > 0x7fffffffL) return ERROR_UNSUPPORTED;
+  CallScratch room(2, p.splits > 1 ? (size_t)p.splits * 2 * p.M * p.N * sizeof(float) : 0);
+  p.part = (float*)room.p;
+  if (p.splits > 1 && !p.part) return CUDA_ERROR;
   p.stage_tx = 2 * (32 * 1024 + bn * 128) + (uint32_t)take_injected_bytes();
+  int err;
   switch (bn) {
-    case 256: return launch_pairs(k_gated_tc<256>, p, tiles);
-    case 128: return launch_pairs(k_gated_tc<128>, p, tiles);
-    case 64: return launch_pairs(k_gated_tc<64>, p, tiles);
+    case 256: err = launch_pairs(k_gated_tc<256>, p, tiles); break;
+    case 128: err = launch_pairs(k_gated_tc<128>, p, tiles); break;
+    case 64: err = launch_pairs(k_gated_tc<64>, p, tiles); break;
+    default: err = launch_pairs(k_gated_tc<32>, p, tiles);
   }
-  return launch_pairs(k_gated_tc<32>, p, tiles);
+  if (err || p.splits == 1) return err;
+  long blocks = ((long)p.M * p.N + 255) / 256;
+  if (blocks > 8L * sm_count()) blocks = 8L * sm_count();
+#define FINISH(ACT) case ACT: (void)launch_dependent(k_gated_finish<ACT>, dim3((unsigned)blocks), dim3(256), 0, stream(), p); break
+  switch (p.activation) { FINISH(kLinear); FINISH(kLogistic); FINISH(kRelu); FINISH(kSilu); FINISH(kGelu); }
+#undef FINISH
+  return check_launch();
 }
 
 int plane_products(const PlaneProduct* f, int nproducts) {
