@@ -909,7 +909,7 @@ class GatedPlanes(object):
     def __init__(self, gate_w, up_w):
         if gate_w.shape != up_w.shape:
             raise CUDAMatException("Incompatible matrix dimensions.")
-        self.gate, self.up, self.scales = AuxMatrix(gate_w.shape), AuxMatrix(up_w.shape), empty((2, gate_w.shape[1]))
+        self.scales, self.gate, self.up = carve([(2, gate_w.shape[1])], aux=[gate_w.shape, up_w.shape])
         self.fill(gate_w, up_w)
 
     def fill(self, gate_w, up_w):

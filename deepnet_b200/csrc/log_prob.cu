@@ -451,6 +451,10 @@ int log_prob_deriv(cudamat* logits, cudamat* tokens, cudamat* stats, cudamat* gr
   if (!same_shape(logits, target) || stats->size[0] != 2 || stats->size[1] != w || (grad && !tokens) || (grad_entropy && !entropy))
     return ERROR_INCOMPATIBLE_DIMENSIONS;
   if (h == 0 || w == 0) return 0;
+  if (h > (1 << 24)) {
+    set_error("a float32 does not hold every token of a column");
+    return ERROR_UNSUPPORTED;
+  }
   auto at = [](cudamat* v) { return v ? v->data_device : nullptr; };
   const float* z = logits->data_device;
   float* dz = target->data_device;

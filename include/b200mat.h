@@ -329,7 +329,7 @@ int dropout_scaled(rnd_struct* rnd_state, cudamat* mat, cudamat* add, cudamat* t
 int log_prob(cudamat* logits, cudamat* tokens, cudamat* target, cudamat* entropy, cudamat* stats, cudamat* top, cudamat* top_tokens);
 /* target (may be logits) = gradient of the logits, from grad (1 x N, or null), the gradient of log_prob's target, and grad_entropy
  * (1 x N, or null; with entropy as log_prob gave it), that of its entropy.  A column whose gradients are 0 gives 0 whatever its
- * logits and token are, and so does one of -inf alone. */
+ * logits and token are, and so does one of -inf alone.  V <= 2^24. */
 int log_prob_deriv(cudamat* logits, cudamat* tokens, cudamat* stats, cudamat* grad, cudamat* entropy, cudamat* grad_entropy, cudamat* target);
 
 /* Library control. */

@@ -95,6 +95,8 @@ def test_log_prob_deriv_refuses():
     assert f(z(), row(), st(), row(), None, row(), z()) == DIMENSIONS              # a gradient of entropies that are not given
     assert f(z(trans=1), row(), st(), row(), None, None, z()) == TRANSPOSED
     assert f(z(), row(), st(), row(), None, None, z(on_device=0)) == NOT_ON_DEVICE
+    long = lambda: mat((1 << 24) + 1, 6)
+    assert f(long(), row(), st(), row(), None, None, long()) == UNSUPPORTED
 
 
 def test_gated_product_refuses():
