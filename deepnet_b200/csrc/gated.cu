@@ -432,10 +432,14 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
   }
   if (H == 0 || N == 0) return 0;
   auto at = [](cudamat* m) { return m ? m->data_device : nullptr; };
-  if (N <= kFewCases && gemm_path() == 0) {
+  // Of large layers the tensor cores read planes faster from five cases on (2048 x 8192, 8 cases: 34 us, 62 without planes, 4 cases 33
+  // and 43), and split weights that do not start on 16 bytes and then read them (2047 x 8191, 7 cases: 85 us, 161 without).
+  const bool on_groups = V % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device);
+  const bool planes_first = (long)V * H >= 1L << 22 && ((gate_planes && N > 4) || (!on_groups && N > 3));
+  if (N <= kFewCases && gemm_path() == 0 && !planes_first) {
     const GatedArgs a = {gate_w->data_device, up_w->data_device, mat->data_device, at(gate_bias), at(up_bias),
                          at(gate),            at(up),            target->data_device, V, H, N};
-    const bool vec = V % 4 == 0 && on16(a.wg) && on16(a.wu) && on16(a.x), block = H < 16L * sm_count() && V >= 512;
+    const bool vec = on_groups, block = H < 16L * sm_count() && V >= 512;
     const dim3 grid(block ? H : (H + 7) / 8);
 #define FEW(CASES)                                                                                                                \
   do {                                                                                                                            \
@@ -516,13 +520,13 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     return 0;
   }
   const bool biases = grad_gate_bias || grad_up_bias, weights = grad_gate_w || grad_up_w;
-  // On planes, or as four products of the matrices themselves (`dot`), which read large weights faster for few cases and spend less
-  // on tiny layers, but take matrices that TMA cannot address behind copies.  Microseconds, planes / dot: 256 x 256, 32 cases 33 / 28;
-  // 784 x 500, 100 cases 41 / 40; 1024 x 1024, 128 cases 42 / 52; 2048 x 8192, 64 cases 190 / 149, 256 cases 228 / 233, 4096 cases
-  // 1402 / 2462; 301 x 301, 301 cases 43 / 61; 1357 x 601, 203 cases 42 / 103.
+  // On planes, or as four products of the matrices themselves (`dot`), which read large weights faster for few cases but take
+  // matrices that TMA cannot address behind copies.  Microseconds, planes / dot: 256 x 256, 32 cases 18 / 28; 784 x 500, 100 cases
+  // 27 / 40; 1024 x 1024, 128 cases 34 / 52; 2048 x 8192, 64 cases 167 / 149, 256 cases 209 / 233, 4096 cases 1385 / 2462; 301 x 301,
+  // 301 cases 25 / 61; 1357 x 601, 203 cases 31 / 103.
   const bool aligned = V % 4 == 0 && H % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device) &&
                        on16(gate->data_device) && on16(up->data_device);
-  const bool few = aligned && !gate_planes && N < 256 && (long)V * H >= 1L << 22;
+  const bool few = aligned && !gate_planes && N < 128 && (long)V * H >= 1L << 22;
   const bool large = (long)V * H * N >= 1L << 16 && !few;
   const bool tc = V > 0 && (weights || grad_mat) && gemm_path() != 2 && (large || gemm_path() == 1) && tma_available();
   const int cases = gated_deriv_cases(N), blocks = (N + cases - 1) / cases;
