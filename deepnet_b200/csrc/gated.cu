@@ -2,6 +2,8 @@
 // and the derivative.  Weights are inputs x units, as an edge's; x is inputs x cases.
 //   G = Wg' x + bg,  U = Wu' x + bu,  y = act(G) U
 //   dU = dy act(G),  dG = dy U act'(G),  dx = Wg dG + Wu dU,  dWg = x dG',  dWu = x dU',  dbg, dbu: row sums of dG, dU
+#include <initializer_list>
+
 #include "gated.cuh"
 #include "gemm.cuh"
 
@@ -343,6 +345,20 @@ int weights_ok(const cudamat* gate_w, const cudamat* up_w) {
   if (gate_w->is_trans || up_w->is_trans) return ERROR_TRANSPOSED;
   return same_shape(gate_w, up_w) ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
 }
+// Whether something that is written lies over anything else: the first `written` matrices may lie over none.
+bool overlapping(std::initializer_list<const cudamat*> mats, int written) {
+  for (int i = 0; i < written; i++)
+    for (int j = i + 1; j < (int)mats.size(); j++) {
+      const cudamat *a = mats.begin()[i], *b = mats.begin()[j];
+      if (!a || !b || numel(a) == 0 || numel(b) == 0) continue;
+      const uintptr_t x = (uintptr_t)a->data_device, y = (uintptr_t)b->data_device;
+      if (x < y + 4 * numel(b) && y < x + 4 * numel(a)) {
+        set_error("a result may not lie over another argument");
+        return true;
+      }
+    }
+  return false;
+}
 // Planes of both weights: all three, on 16 bytes.
 int planes_ok(const cudamat* w, const cudamat* gate_planes, const cudamat* up_planes, const cudamat* scales) {
   if (!gate_planes || !up_planes || !scales) return ERROR_INCOMPATIBLE_DIMENSIONS;
@@ -410,6 +426,7 @@ int gated_planes(cudamat* gate_w, cudamat* up_w, cudamat* gate_planes, cudamat* 
   if (err) return err;
   const int V = gate_w->size[0], H = gate_w->size[1];
   if (V == 0 || H == 0) return 0;
+  if (overlapping({gate_planes, up_planes, scales, gate_w, up_w}, 3)) return ERROR_UNSUPPORTED;
   const SplitJob jobs[2] = {{gate_w->data_device, (uint16_t*)gate_planes->data_device, scales->data_device, 2, H},
                             {up_w->data_device, (uint16_t*)up_planes->data_device, scales->data_device + 1, 2, H}};
   return split_columns(jobs, 2, V);
@@ -431,6 +448,7 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
     return ERROR_UNSUPPORTED;
   }
   if (H == 0 || N == 0) return 0;
+  if (overlapping({target, gate, up, mat, gate_w, up_w, gate_bias, up_bias, gate_planes, up_planes, scales}, 3)) return ERROR_UNSUPPORTED;
   auto at = [](cudamat* m) { return m ? m->data_device : nullptr; };
   // Of large layers the tensor cores read planes faster from five cases on (2048 x 8192, 8 cases: 34 us, 62 without planes, 4 cases 33
   // and 43), and split weights that do not start on 16 bytes and then read them (2047 x 8191, 7 cases: 85 us, 161 without).
@@ -513,6 +531,9 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     set_error("no such activation");
     return ERROR_UNSUPPORTED;
   }
+  if (overlapping({gate, up, grad_mat, grad_gate_w, grad_up_w, grad_gate_bias, grad_up_bias, deriv, gate_w, up_w, mat, gate_planes, up_planes,
+                   scales}, 7))
+    return ERROR_UNSUPPORTED;
   if (N == 0 || H == 0) {           // sums over no cases, or no units
     for (cudamat* m : {grad_gate_bias, grad_up_bias, grad_gate_w, grad_up_w, grad_mat})
       if (m && numel(m) && cudaMemsetAsync(m->data_device, 0, sizeof(float) * numel(m), stream()) != cudaSuccess)

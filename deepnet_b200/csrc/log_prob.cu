@@ -122,9 +122,9 @@ __device__ __forceinline__ void store_group(float* column, int r, int h, const f
   }
 }
 
-// A float's bits in the floats' order, and back (0: below all).
+// A float's bits in the floats' order, both zeros alike, and back (0: below all).
 __device__ __forceinline__ uint32_t ordered(float v) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = __float_as_uint(v + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }

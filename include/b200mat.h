@@ -302,7 +302,7 @@ int layer_norm_deriv(cudamat* deriv, cudamat* mat, cudamat* stats, cudamat* gain
 
 /* A gated layer: target (H x N) = act(gate_w' mat + gate_bias) * (up_w' mat + up_bias), weights V x H, mat V x N, biases (one value a
  * unit) or null; activation 0 none, 1 logistic, 2 max(0, g), 3 g logistic(g), 4 g Phi(g).  gate and up (H x N, both or neither) receive
- * the sums the activation is taken of, for the derivative. */
+ * the sums the activation is taken of, for the derivative.  No result of this call or the next may lie over another argument. */
 int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bias, cudamat* up_bias, int activation,
                   cudamat* gate_planes, cudamat* up_planes, cudamat* scales, cudamat* gate, cudamat* up, cudamat* target);
 /* The weights' form for the tensor cores, for layers that run many times between changes of their weights: gate_planes, up_planes

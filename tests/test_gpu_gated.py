@@ -380,3 +380,18 @@ def test_two_recorded_derivatives_share_no_scratch(cm):
         for k, v in s["out"].items():
             assert np.array_equal(get(v), w[k]), k
     assert cm.read_status() == 0
+
+
+def test_results_of_more_than_2_to_31_elements(cm):
+    rng = np.random.default_rng(6)
+    V, H, N = 64, 65536, 32800
+    wg, wu = (cm.CUDAMatrix((rng.standard_normal((V, H)) / 8).astype(np.float32)) for _ in range(2))
+    last = rng.standard_normal((V, 300)).astype(np.float32)
+    x, y = cm.empty((V, N)), cm.empty((H, N))
+    x.slice(N - 300, N).assign(cm.CUDAMatrix(last))
+    cm.gated_product(wg, wu, x, y, activation="relu")
+    want = cm.gated_product(wg, wu, cm.CUDAMatrix(last), activation="relu")
+    assert np.array_equal(get(y.slice(N - 300, N)), get(want))            # a case's sums do not depend on the others
+    assert (get(y.slice(0, 2)) == 0).all()
+    y.free_device_memory()
+    assert cm.read_status() == 0

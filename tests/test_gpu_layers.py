@@ -385,6 +385,19 @@ def test_columns_without_a_distribution(cm):
         assert np.isnan(get(gz.log_prob(cm.CUDAMatrix(np.full((1, 8), bad))))).all()
 
 
+@pytest.mark.parametrize("h", [5, 40, 700, 5000])
+def test_both_zeros_are_one_logit(cm, h):
+    """Of equal logits the lower number, and 0 and -0 are equal."""
+    z = np.full((h, 3), -1.0, np.float32)
+    z[[0, h // 2, h - 1], 0] = [-0.0, 0.0, -0.0]
+    z[[1, h // 2, h - 1], 1] = [0.0, -0.0, 0.0]
+    z[h - 2:, 2] = -0.0
+    z[0, 2] = 0.0
+    top, tops = cm.empty((3, 3)), cm.empty((3, 3))
+    cm.CUDAMatrix(z).log_prob(top=top, top_tokens=tops)
+    assert np.array_equal(get(tops), np.array([[0, h // 2, h - 1], [1, h // 2, h - 1], [0, h - 2, h - 1]], np.float32).T)
+
+
 @pytest.mark.parametrize("off", [1, 2, 3])
 def test_logits_that_start_anywhere(cm, off):
     rng = np.random.default_rng(off)
@@ -479,6 +492,49 @@ def test_two_recorded_passes_share_no_scratch(cm):
     for s, w in zip(sets, want):
         for n, v in zip(names, w):
             assert np.array_equal(get(s[n]), v), n
+
+
+def test_matrices_of_more_than_2_to_31_elements(cm):
+    """Their last columns as their own matrices give them."""
+    h, w = 65536, 32800
+    big = cm.empty((h, w))
+    rng = np.random.default_rng(1)
+    last = rng.standard_normal((h, 2)).astype(np.float32)
+
+    def refill():
+        big.slice(w - 2, w).assign(cm.CUDAMatrix(last))
+    refill()
+    lp, st, top, tops, t = cm.empty((1, w)), cm.empty((2, w)), cm.empty((4, w)), cm.empty((4, w)), cm.CUDAMatrix(np.full((1, w), 7.0))
+    big.log_prob(t, target=lp, stats=st, top=top, top_tokens=tops)
+    small, s1, p1, i1, t1 = cm.CUDAMatrix(last), cm.empty((2, 2)), cm.empty((4, 2)), cm.empty((4, 2)), cm.CUDAMatrix(np.full((1, 2), 7.0))
+    l1 = small.log_prob(t1, stats=s1, top=p1, top_tokens=i1)
+    # (sums in another grouping: within 2 (h / 32 + 100) roundings of values of some 12)
+    tol = dict(rtol=0, atol=2 * (h / 32 + 100) * U * 12)
+    np.testing.assert_allclose(get(lp)[:, -2:], get(l1), **tol)
+    assert np.array_equal(get(tops)[:, -2:], get(i1)) and abs(get(lp)[0, 0] + np.log(h)) < 1e-4
+    g = cm.CUDAMatrix(np.ones((1, w)))
+    big.log_prob_deriv(t, st, g)
+    small.log_prob_deriv(t1, s1, cm.CUDAMatrix(np.ones((1, 2))))
+    np.testing.assert_allclose(get(big.slice(w - 2, w)), get(small), **tol)
+    refill()
+    small = cm.CUDAMatrix(last)
+    big.dropout_scaled(0.5, key=(3, 4))
+    cm.set_rng_column_offset(w - 2)
+    try:
+        small.dropout_scaled(0.5, key=(3, 4))
+    finally:
+        cm.set_rng_column_offset(0)
+    assert np.array_equal(get(big.slice(w - 2, w)), get(small))
+    refill()
+    small = cm.CUDAMatrix(last)
+    st1, gain = cm.empty((2, 2)), cm.empty((h, 1))
+    big.layer_norm(stats=st)
+    small.layer_norm(stats=st1)
+    assert np.array_equal(get(big.slice(w - 2, w)), get(small)) and np.array_equal(get(st)[:, -2:], get(st1))
+    big.layer_norm_deriv(big, st, grad_gain=gain)       # (any gradient will do: the normalised values themselves)
+    small.layer_norm_deriv(small, st1)
+    assert np.array_equal(get(big.slice(w - 2, w)), get(small))
+    big.free_device_memory()
 
 
 def test_calls_on_another_stream(cm):

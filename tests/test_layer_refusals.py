@@ -9,10 +9,15 @@ from deepnet_b200 import b200mat as cm
 DIMENSIONS, TRANSPOSED, NOT_ON_DEVICE, UNSUPPORTED = -1, -5, -8, -9
 
 
-def mat(rows, cols, on_device=1, trans=0):
+_place = [1 << 20]
+
+
+def mat(rows, cols, on_device=1, trans=0, at=None):
+    """A handle of memory that nobody has, each somewhere else (or `at` an address)."""
     m = cm.cudamat()
     m.size[0], m.size[1], m.on_device, m.is_trans = rows, cols, on_device, trans
-    m.data_device = ct.cast(0, ct.POINTER(ct.c_float))
+    m.data_device = ct.cast(_place[0] if at is None else at, ct.POINTER(ct.c_float))
+    _place[0] += (4 * rows * cols + 255) // 256 * 256
     return ct.pointer(m)
 
 
@@ -123,7 +128,7 @@ def test_gated_product_refuses():
         planes[i] = bad
         assert f(w(), w(), x(), planes=planes) == err and (fill(planes) == err)
     planes = good()
-    planes[1].contents.data_device = ct.cast(8, ct.POINTER(ct.c_float))
+    planes[1] = mat(16, 7, at=(1 << 40) + 8)
     assert f(w(), w(), x(), planes=planes) == UNSUPPORTED and fill(planes) == UNSUPPORTED
     with pytest.raises(cm.CUDAMatException):
         cm._gated_activation("softmax")
@@ -141,3 +146,28 @@ def test_gated_product_deriv_refuses():
     assert f(gate=mat(7, 5, trans=1)) == TRANSPOSED and f(out=(None, None, mat(9, 7, trans=1), None, None)) == TRANSPOSED
     assert f(x=mat(9, 5, on_device=0)) == NOT_ON_DEVICE and f(out=(None, None, None, None, mat(7, 1, on_device=0))) == NOT_ON_DEVICE
     assert f(act=9) == UNSUPPORTED
+
+
+def test_results_may_not_lie_over_other_arguments():
+    """Square shapes, where every matrix could stand for every other; one byte in common is enough."""
+    sq = lambda at: mat(8, 8, at=at)
+    names = ["wg", "wu", "x", "gate", "up", "y"]
+    for i, a in enumerate(names):
+        for b in names[:i]:
+            if a in ("wg", "wu", "x") and b in ("wg", "wu", "x"):
+                continue
+            place = {n: (1 << 30) + 4096 * k for k, n in enumerate(names)}
+            place[a] = place[b] + 252
+            m = {n: sq(p) for n, p in place.items()}
+            assert cm._lib.gated_product(m["wg"], m["wu"], m["x"], None, None, ct.c_int(1), None, None, None, m["gate"], m["up"],
+                                         m["y"]) == UNSUPPORTED, (a, b)
+    names = ["dy", "wg", "wu", "x", "gate", "up", "dx", "dwg", "dwu"]
+    for i, a in enumerate(names):
+        for b in names[:i]:
+            if i < 4:
+                continue
+            place = {n: (1 << 30) + 4096 * k for k, n in enumerate(names)}
+            place[a] = place[b] - 252
+            m = {n: sq(p) for n, p in place.items()}
+            assert cm._lib.gated_product_deriv(m["dy"], m["gate"], m["up"], m["wg"], m["wu"], m["x"], ct.c_int(1), None, None, None, m["dx"],
+                                               m["dwg"], m["dwu"], None, None) == UNSUPPORTED, (a, b)
