@@ -92,8 +92,12 @@ __global__ void __launch_bounds__(256) k_gated_few(const GatedArgs a, int activa
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const long u = kWarps > 1 ? (long)blockIdx.x : (long)blockIdx.x * 8 + wid;
   if (u >= a.H) return;
-  constexpr int kBatch = kVec == 4 ? 4 : 8;
+  // groups on their way: what the registers of kN cases leave (2048 x 8192, 8 cases: 4 groups 83 us, 1 group 52)
+  constexpr int kBatch = kN <= 2 ? (kVec == 4 ? 4 : 8) : kN == 4 ? (kVec == 4 ? 2 : 8) : (kVec == 4 ? 1 : 4);
   const float *wg = a.wg + u * a.V, *wu = a.wu + u * a.V;
+  const float* xs[kN];
+#pragma unroll
+  for (int n = 0; n < kN; n++) xs[n] = a.x + (n < a.N ? (long)n * a.V : 0);
   float sum[2 * kN];
 #pragma unroll
   for (int i = 0; i < 2 * kN; i++) sum[i] = 0.0f;
@@ -111,21 +115,27 @@ __global__ void __launch_bounds__(256) k_gated_few(const GatedArgs a, int activa
         for (int j = 0; j < kVec; j++) g[b][j] = w[b][j] = 0.0f;
       }
     }
+    // (no branch around a load: cases beyond the last read the first again, a group beyond the last is 0)
 #pragma unroll
     for (int b = 0; b < kBatch; b++) {
       const int i = base + b * step;
-      if (i >= items) continue;
+      float x[kN][kVec];
 #pragma unroll
       for (int n = 0; n < kN; n++) {
-        if (n >= a.N) continue;
-        float x[kVec];
-        load<kVec>(a.x + (long)n * a.V + (long)i * kVec, x);
+        if (i < items) {
+          load<kVec>(xs[n] + (long)i * kVec, x[n]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kVec; j++) {
-          sum[2 * n] = fmaf(g[b][j], x[j], sum[2 * n]);
-          sum[2 * n + 1] = fmaf(w[b][j], x[j], sum[2 * n + 1]);
+          for (int j = 0; j < kVec; j++) x[n][j] = 0.0f;
         }
       }
+#pragma unroll
+      for (int n = 0; n < kN; n++)
+#pragma unroll
+        for (int j = 0; j < kVec; j++) {
+          sum[2 * n] = fmaf(g[b][j], x[n][j], sum[2 * n]);
+          sum[2 * n + 1] = fmaf(w[b][j], x[n][j], sum[2 * n + 1]);
+        }
     }
   }
 #pragma unroll
@@ -450,8 +460,8 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
   if (H == 0 || N == 0) return 0;
   if (overlapping({target, gate, up, mat, gate_w, up_w, gate_bias, up_bias, gate_planes, up_planes, scales}, 3)) return ERROR_UNSUPPORTED;
   auto at = [](cudamat* m) { return m ? m->data_device : nullptr; };
-  // Of large layers the tensor cores read planes faster from five cases on (2048 x 8192, 8 cases: 34 us, 62 without planes, 4 cases 33
-  // and 43), and split weights that do not start on 16 bytes and then read them (2047 x 8191, 7 cases: 85 us, 161 without).
+  // Of large layers the tensor cores read planes faster from five cases on (2048 x 8192, 8 cases: 34 us, 52 without planes, 4 cases 33
+  // and 35), and split weights that do not start on 16 bytes and then read them (2047 x 8191, 7 cases: 85 us, 161 without).
   const bool on_groups = V % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device);
   const bool planes_first = (long)V * H >= 1L << 22 && ((gate_planes && N > 4) || (!on_groups && N > 3));
   if (N <= kFewCases && gemm_path() == 0 && !planes_first) {
