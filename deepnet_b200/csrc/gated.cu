@@ -460,10 +460,10 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
   if (H == 0 || N == 0) return 0;
   if (overlapping({target, gate, up, mat, gate_w, up_w, gate_bias, up_bias, gate_planes, up_planes, scales}, 3)) return ERROR_UNSUPPORTED;
   auto at = [](cudamat* m) { return m ? m->data_device : nullptr; };
-  // Of large layers the tensor cores read planes faster from five cases on (2048 x 8192, 8 cases: 34 us, 52 without planes, 4 cases 33
-  // and 35), and split weights that do not start on 16 bytes and then read them (2047 x 8191, 7 cases: 85 us, 161 without).
+  // Of large layers the tensor cores read planes faster from five cases on: 2048 x 8192, 8 cases 34 us, 52 without planes (83 with the
+  // split before them), 4 cases 33 and 35.
   const bool on_groups = V % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device);
-  const bool planes_first = (long)V * H >= 1L << 22 && ((gate_planes && N > 4) || (!on_groups && N > 3));
+  const bool planes_first = gate_planes && N > 4 && (long)V * H >= 1L << 22;
   if (N <= kFewCases && gemm_path() == 0 && !planes_first) {
     const GatedArgs a = {gate_w->data_device, up_w->data_device, mat->data_device, at(gate_bias), at(up_bias),
                          at(gate),            at(up),            target->data_device, V, H, N};
