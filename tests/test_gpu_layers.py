@@ -268,7 +268,7 @@ def words_bounds(z, lp, p, ent, d, s):
 
 
 WORDS = [(1, 1), (2, 3), (7, 5), (32, 4), (33, 1), (100, 64), (255, 30), (256, 1), (1000, 2), (1001, 5), (10000, 1), (10000, 37), (4099, 301),
-         (50021, 6), (100000, 1), (64, 6000)]
+         (50021, 6), (100000, 1), (64, 6000), (600001, 2)]
 
 
 def ranked(z, k):
