@@ -131,6 +131,7 @@ __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(
 
 constexpr int kCandidates = 512;       // of a block's columns together
 constexpr int kChunks = 2048;          // chunks (a warp's 128 logits) whose maxima a block keeps
+static_assert(kChunks * sizeof(uint32_t) == 32 * kMostTop * sizeof(Top), "a column's share of the maxima is its lists'");
 
 // A column is read by `warps` of the block's warps (a power of two), the next kBatch groups of a thread on their way while it works
 // on some.
@@ -139,7 +140,8 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
   constexpr int kBatch = 4;
   __shared__ Sums sums[32];
   __shared__ uint32_t bounds[32];
-  // (the lists come after the maxima's last use)
+  // A column's own share of it, whether maxima or lists: the lists come after its maxima's last use, but other columns of the block
+  // may still be at theirs.
   __shared__ union {
     uint32_t maxima[kTop ? kChunks : 1];
     Top lists[kTop ? 32 * kMostTop : 1];
@@ -200,6 +202,7 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
   // this warp's chunks' maxima: chunk b of its round i at maxima[(i * kBatch + b) * warps + wid]
   const int most = kChunks / groups;
   uint32_t* const maxima = shared.maxima + (kTop ? group * most : 0);
+  Top* const lists = shared.lists + (kTop ? group * (32 * kMostTop / groups) : 0);       // one a warp: warps x groups is 32 at most
   const bool kept = ((items + kBatch * threads - 1) / (kBatch * threads)) * kBatch * warps <= most;
   Sums s = {-INFINITY, 0.0f, 0.0f};
   float m = kLowest;                                   // s.m, finite where nothing but -inf was seen
@@ -328,11 +331,13 @@ __global__ void __launch_bounds__(1024) k_log_prob(const LogProbArgs a, int warp
     float kv = -INFINITY;
     int ki = 0x7fffffff;
     each([](float, const float (&)[kBatch][4], int) { return true; }, [&](float v, int i) { offer(list, a.k, v, i >= 0 && i < a.h ? i : 0x7fffffff, kv, ki); });
-    if (lane < a.k) shared.lists[(first_warp + wid) * kMostTop + lane] = list;
-    meet();
-    if (wid) return;
+    if (warps > 1) {
+      if (lane < a.k) lists[wid * kMostTop + lane] = list;
+      meet();
+      if (wid) return;
+    }
     for (int x = 1; x < warps; x++) {
-      const Top other = lane < a.k ? shared.lists[(first_warp + x) * kMostTop + lane] : Top{-INFINITY, 0x7fffffff};
+      const Top other = lane < a.k ? lists[x * kMostTop + lane] : Top{-INFINITY, 0x7fffffff};
       offer(list, a.k, other.v, other.i, kv, ki);
     }
     if (lane < a.k) put(lane, list);

@@ -353,6 +353,41 @@ def test_log_probabilities_entropy_likeliest_and_gradient(cm, shape, kind):
     within(get(over), -p * q * (flp + H) * (p > 0), 1.01 * bound)
 
 
+@pytest.mark.parametrize("k", [5, 20, 32])
+@pytest.mark.parametrize("h", [300, 512, 5000, 30000])
+@pytest.mark.parametrize("w", [260, 131, 67, 33])
+def test_likeliest_words_of_columns_that_share_a_block(cm, h, w, k):
+    """Columns that find their words in one look beside columns that need sorted lists (equal logits, fewer words than are asked for,
+    words in order), in any order: none may touch what another still reads.  On eight SMs these numbers of columns are read by one
+    warp each, by two, by four and by eight, where a column is long enough."""
+    rng = np.random.default_rng(h + 7 * w + k)
+    z = (3 * rng.standard_normal((h, w))).astype(np.float32)
+    kind = rng.integers(0, 5, w)
+    z[:, kind == 1] = 1.0                                           # all equal
+    some = np.flatnonzero(kind == 2)
+    z[:, some] = -np.inf
+    for c in some:
+        z[rng.integers(0, h, 3), c] = rng.standard_normal(3)        # at most three words left
+    z[:, kind == 3] = np.sort(z[:, kind == 3], axis=0)
+    z[:, kind == 4] = np.round(z[:, kind == 4])
+    want = ranked(z, k).astype(np.float32)
+    gz, top, tops = cm.CUDAMatrix(z), cm.empty((k, w)), cm.empty((k, w))
+    cm.set_sm_limit(8)
+    try:
+        for _ in range(5):
+            tops.assign(-1)
+            gz.log_prob(top=top, top_tokens=tops)
+            assert np.array_equal(get(tops), want)
+    finally:
+        cm.set_sm_limit(0)
+    best = np.take_along_axis(z, want.astype(np.int64), 0)
+    fell = np.isneginf(best)
+    assert np.array_equal(np.isneginf(get(top)), fell)
+    # log p differs from column to column by one number alone: differences of logits, each off by a few roundings of values up to 40
+    got = np.where(fell, 0, get(top) - get(top)[:1])
+    np.testing.assert_allclose(got, np.where(fell, 0, best - best[:1]), rtol=0, atol=4 * 40 * U)
+
+
 def test_columns_without_a_distribution(cm):
     h = 300
     z = np.random.default_rng(2).standard_normal((h, 8)).astype(np.float32)
