@@ -904,22 +904,23 @@ def _gated_activation(name):
 
 class GatedPlanes(object):
     """A gated layer's weights in the form its tensor-core products read (`gated_planes` in b200mat.h), for layers that run many times
-    between changes of their weights: as of this call, or of the last `fill`."""
+    between changes of their weights: as of this call, or of the last `fill`, which has to follow every change of them (few cases
+    read the weights themselves).  Every weight is kept whole, in 6 bytes."""
 
     def __init__(self, gate_w, up_w):
         if gate_w.shape != up_w.shape:
             raise CUDAMatException("Incompatible matrix dimensions.")
-        self.scales, self.gate, self.up = carve([(2, gate_w.shape[1])], aux=[gate_w.shape, up_w.shape])
+        self.gate, self.up, self.low = carve([], aux=[gate_w.shape] * 3)
         self.fill(gate_w, up_w)
 
     def fill(self, gate_w, up_w):
         """After the weights have changed."""
-        _check(_lib.gated_planes(gate_w.p_mat, up_w.p_mat, self.gate.p_mat, self.up.p_mat, self.scales.p_mat))
+        _check(_lib.gated_planes(gate_w.p_mat, up_w.p_mat, self.gate.p_mat, self.up.p_mat, self.low.p_mat))
         return self
 
 
 def _planes(planes):
-    return (planes.gate.p_mat, planes.up.p_mat, planes.scales.p_mat) if planes is not None else (None, None, None)
+    return (planes.gate.p_mat, planes.up.p_mat, planes.low.p_mat) if planes is not None else (None, None, None)
 
 
 def gated_product(gate_w, up_w, mat, target=None, activation="logistic", gate_bias=None, up_bias=None, gate=None, up=None, planes=None):

@@ -21,20 +21,6 @@ struct GatedArgs {
   int V, H, N;
 };
 
-template <int kVec>
-__device__ __forceinline__ void load(const float* p, float (&v)[kVec]) {
-  if constexpr (kVec == 4) {
-    const float4 x = *reinterpret_cast<const float4*>(p);
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-  } else {
-    v[0] = *p;
-  }
-}
-template <int kVec>
-__device__ __forceinline__ void store(float* p, const float (&v)[kVec]) {
-  if constexpr (kVec == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  else *p = v[0];
-}
 // 64 units by 64 cases a block of 256 threads, four by four of both products a thread, full fp32 multiply-adds.
 template <int kAct>
 __global__ void __launch_bounds__(256) k_gated_simt(const GatedArgs a) {
@@ -181,14 +167,9 @@ __global__ void __launch_bounds__(256) k_gated_few(const GatedArgs a, int activa
 }
 
 // ---- the derivative's elementwise part ------------------------------------------------------
-// A thread takes kVec units of some cases, one case after another: the units' sums and maxima stay in registers.  Bound by HBM:
-// 20 bytes a unit and case for the gradients, 8 + 16 for their planes.
+// A thread takes kVec units of some cases, one case after another: the units' sums stay in registers.  Bound by HBM: 20 bytes a unit and
+// case for the gradients, 12 more for their parts.
 constexpr int kMostCases = 64, kDerivThreads = 128;
-
-__device__ __forceinline__ uint32_t magnitude(float v) {      // bits of finite magnitudes, in their order
-  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
-}
 
 template <int kAct, int kVec>
 __global__ void __launch_bounds__(kDerivThreads) k_gated_deriv(const GatedDeriv a) {
@@ -196,24 +177,16 @@ __global__ void __launch_bounds__(kDerivThreads) k_gated_deriv(const GatedDeriv 
   grid_dependency_wait();
   const int blocks_u = (a.H + kDerivThreads * kVec - 1) / (kDerivThreads * kVec), ub = blockIdx.x % blocks_u, cb = blockIdx.x / blocks_u;
   const int r = (ub * kDerivThreads + threadIdx.x) * kVec;
-  const bool in = r < a.H;
+  if (r >= a.H) return;
   const int c1 = min(a.N, (cb + 1) * a.cases);
-  float sg[kVec] = {}, su[kVec] = {}, wg[kVec], wu[kVec];
-  uint32_t mg[kVec] = {}, mu[kVec] = {};
-#pragma unroll
-  for (int j = 0; j < kVec; j++) {
-    wg[j] = in && a.w_inv ? a.w_inv[2L * (r + j)] : 0.0f;
-    wu[j] = in && a.w_inv ? a.w_inv[2L * (r + j) + 1] : 0.0f;
-  }
+  float sg[kVec] = {}, su[kVec] = {};
 #pragma unroll 2
   for (int c = cb * a.cases; c < c1; c++) {
     const long at = (long)c * a.H + r;
-    float d[kVec] = {}, g[kVec] = {}, u[kVec] = {};
-    if (in) {
-      load<kVec>(a.dy + at, d);
-      load<kVec>(a.gate + at, g);
-      load<kVec>(a.up + at, u);
-    }
+    float d[kVec], g[kVec], u[kVec];
+    load<kVec>(a.dy + at, d);
+    load<kVec>(a.gate + at, g);
+    load<kVec>(a.up + at, u);
 #pragma unroll
     for (int j = 0; j < kVec; j++) {
       float slope;
@@ -223,122 +196,42 @@ __global__ void __launch_bounds__(kDerivThreads) k_gated_deriv(const GatedDeriv 
       sg[j] += g[j];
       su[j] += u[j];
     }
-    if (in) {
-      store<kVec>(a.gate + at, g);
-      store<kVec>(a.up + at, u);
-    }
-    if (a.token_max) {
-      const float xi = a.x_inv[c];
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < kVec; j++) {
-        m = max(m, max(magnitude(g[j] * wg[j]), magnitude(u[j] * wu[j])));
-        mg[j] = max(mg[j], magnitude(g[j] * xi));
-        mu[j] = max(mu[j], magnitude(u[j] * xi));
-      }
-      m = __reduce_max_sync(0xffffffffu, m);
-      if ((threadIdx.x & 31) == 0 && m) atomicMax(a.token_max + c, m);
+    store<kVec>(a.gate + at, g);
+    store<kVec>(a.up + at, u);
+    if (a.parts_g.p) {
+      store_parts<kVec>(a.parts_g, r, c, g);
+      store_parts<kVec>(a.parts_u, r, c, u);
     }
   }
-  if (!in) return;
-  // Maxima, which are the same in any order.  Most blocks come too late to raise one: a look first, at all of them at once.
-  uint32_t seen[2 * kVec];
-#pragma unroll
-  for (int j = 0; j < 2 * kVec; j++) seen[j] = a.token_max ? __ldcg(a.unit_max + 2L * r + j) : 0u;
+  if (!a.part) return;
 #pragma unroll
   for (int j = 0; j < kVec; j++) {
-    if (a.part) {
-      a.part[2L * cb * a.H + r + j] = sg[j];
-      a.part[(2L * cb + 1) * a.H + r + j] = su[j];
-    }
-    if (a.token_max) {
-      if (mg[j] > seen[2 * j]) atomicMax(a.unit_max + 2L * (r + j), mg[j]);
-      if (mu[j] > seen[2 * j + 1]) atomicMax(a.unit_max + 2L * (r + j) + 1, mu[j]);
-    }
+    a.part[2L * cb * a.H + r + j] = sg[j];
+    a.part[(2L * cb + 1) * a.H + r + j] = su[j];
   }
 }
 
-// The blocks' sums, in order: 32 values a block, four threads a value.
-__device__ __forceinline__ void sum_biases(const BiasSums& a, int block) {
+// Sums of dG and dU over all cases: the blocks' of `part` (GatedDeriv) in order, 32 values a block, four threads a value.
+__global__ void __launch_bounds__(kDerivThreads) k_gated_biases(const float* part, int blocks, int H, float* gate, float* up) {
   __shared__ float red[kDerivThreads / 32][33];
+  grid_dependents_launch();
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const long v = (long)block * 32 + lane;
+  const long v = (long)blockIdx.x * 32 + lane;
   float s = 0.0f;
-  if (v < 2L * a.H) {
+  if (v < 2L * H) {
 #pragma unroll 8
-    for (int b = wid; b < a.blocks; b += kDerivThreads / 32) s += a.part[2L * b * a.H + v];
+    for (int b = wid; b < blocks; b += kDerivThreads / 32) s += part[2L * b * H + v];
   }
   red[wid][lane] = s;
   __syncthreads();
-  if (wid || v >= 2L * a.H) return;
+  if (wid || v >= 2L * H) return;
 #pragma unroll
   for (int k = 1; k < kDerivThreads / 32; k++) s += red[k][lane];
-  if (v < a.H) {
-    if (a.gate) a.gate[v] = s;
-  } else if (a.up) {
-    a.up[v - a.H] = s;
-  }
-}
-__global__ void __launch_bounds__(kDerivThreads) k_gated_biases(const BiasSums a) {
-  grid_dependents_launch();
-  grid_dependency_wait();
-  sum_biases(a, blockIdx.x);
-}
-
-__device__ __forceinline__ float power_of(uint32_t max_bits, float* inv) {
-  const int e = (int)f16_exponent(__uint_as_float(max_bits));
-  if (inv) *inv = __int_as_float((127 - e) << 23);
-  return __int_as_float((127 + e) << 23);
-}
-
-template <int kVec>
-__global__ void __launch_bounds__(kDerivThreads) k_gradient_planes(const GradientPlanes a) {
-  grid_dependents_launch();
-  grid_dependency_wait();
-  if ((int)blockIdx.x >= a.grid) {           // the biases' sums ride along
-    sum_biases(a.biases, blockIdx.x - a.grid);
-    return;
-  }
-  const int blocks_u = (a.H + kDerivThreads * kVec - 1) / (kDerivThreads * kVec), ub = blockIdx.x % blocks_u, cb = blockIdx.x / blocks_u;
-  const int r = (ub * kDerivThreads + threadIdx.x) * kVec, lda = aux_rows(a.H);
-  if (r >= a.H) return;
-  const int c1 = min(a.N, (cb + 1) * a.cases);
-  float w[2][kVec], s[2][kVec];
-#pragma unroll
-  for (int k = 0; k < 2; k++)
-#pragma unroll
-    for (int j = 0; j < kVec; j++) {
-      const long i = 2L * (r + j) + k;
-      w[k][j] = a.w_inv[i];
-      s[k][j] = power_of(a.unit_max[i], cb == 0 && a.by_unit[0] ? a.unit_inv + i : nullptr);
-    }
-#pragma unroll 2
-  for (int c = cb * a.cases; c < c1; c++) {
-    const float xi = a.x_inv[c], sc = power_of(a.token_max[c], r == 0 && a.by_case[0] ? a.case_inv + c : nullptr);
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      float v[kVec];
-      load<kVec>((k ? a.up : a.gate) + (long)c * a.H + r, v);
-      auto write = [&](uint16_t* planes, const float (&f)[kVec], const float (&scale)[kVec]) {
-        uint16_t lo[kVec], hi[kVec], *at = planes + (long)c * 2 * lda + r;
-#pragma unroll
-        for (int j = 0; j < kVec; j++) split_f16(v[j] * f[j], scale[j], lo[j], hi[j]);
-        if constexpr (kVec == 4) {
-          *reinterpret_cast<ushort4*>(at) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
-          *reinterpret_cast<ushort4*>(at + lda) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
-        } else {
-          at[0] = lo[0];
-          at[lda] = hi[0];
-        }
-      };
-      float one[kVec];
-#pragma unroll
-      for (int j = 0; j < kVec; j++) one[j] = sc;
-      if (a.by_case[0]) write(a.by_case[k], w[k], one);
-#pragma unroll
-      for (int j = 0; j < kVec; j++) one[j] = xi;
-      if (a.by_unit[0]) write(a.by_unit[k], one, s[k]);
-    }
+  if (v < H) {
+    if (gate) gate[v] = s;
+  } else if (up) {
+    up[v - H] = s;
   }
 }
 
@@ -369,33 +262,37 @@ bool overlapping(std::initializer_list<const cudamat*> mats, int written) {
     }
   return false;
 }
-// Planes of both weights: all three, on 16 bytes.
-int planes_ok(const cudamat* w, const cudamat* gate_planes, const cudamat* up_planes, const cudamat* scales) {
-  if (!gate_planes || !up_planes || !scales) return ERROR_INCOMPATIBLE_DIMENSIONS;
-  if (!gate_planes->on_device || !up_planes->on_device || !scales->on_device) return ERROR_NOT_ON_DEVICE;
-  if (gate_planes->is_trans || up_planes->is_trans || scales->is_trans) return ERROR_TRANSPOSED;
-  const int lda = aux_rows(w->size[0]), H = w->size[1];
-  if (!is(gate_planes, lda, H) || !is(up_planes, lda, H) || !is(scales, 2, H)) return ERROR_INCOMPATIBLE_DIMENSIONS;
-  if (!on16(gate_planes->data_device) || !on16(up_planes->data_device)) {
-    set_error("planes have to start on 16 bytes");
-    return ERROR_UNSUPPORTED;
-  }
+// Parts of both weights: all three matrices, on 16 bytes.
+int planes_ok(const cudamat* w, const cudamat* gate_planes, const cudamat* up_planes, const cudamat* low_planes) {
+  const cudamat* const all[3] = {gate_planes, up_planes, low_planes};
+  for (const cudamat* m : all)
+    if (!m) return ERROR_INCOMPATIBLE_DIMENSIONS;
+  for (const cudamat* m : all)
+    if (!m->on_device) return ERROR_NOT_ON_DEVICE;
+  for (const cudamat* m : all)
+    if (m->is_trans) return ERROR_TRANSPOSED;
+  for (const cudamat* m : all)
+    if (!on16(m->data_device)) {
+      set_error("planes have to start on 16 bytes");
+      return ERROR_UNSUPPORTED;
+    }
+  for (const cudamat* m : all)
+    if (!is(m, aux_rows(w->size[0]), w->size[1])) return ERROR_INCOMPATIBLE_DIMENSIONS;
   return 0;
+}
+// Gate's or up's (`which` 1) parts among them.
+Planes weight_planes(const cudamat* w, const cudamat* planes, const cudamat* low_planes, int which) {
+  const int lda = aux_rows(w->size[0]);
+  return {(uint16_t*)planes->data_device, (uint16_t*)low_planes->data_device + which * lda, 2 * lda, w->size[0], w->size[1]};
 }
 
 }  // namespace
 
 namespace b200 {
-// A block's cases are worked on one after another (0.35 us each), its units' maxima raised at the end: up to 0.09 us for each block
-// that raises the same one.  About 48 blocks of cases.
+// A block's cases are worked on one after another (0.35 us each).  About 48 blocks of cases.
 int gated_deriv_cases(int N) {
   const int cases = (N + 47) / 48;
   return cases > kMostCases ? kMostCases : cases;
-}
-// As many as leave the device eight blocks an SM.
-static int planes_cases(int H, int N) {
-  const long cases = (long)((H + 511) / 512) * N / (8L * sm_count());
-  return cases < 1 ? 1 : cases > kMostCases ? kMostCases : (int)cases;
 }
 static long deriv_grid(int H, int N, int cases, bool vec) {
   const int units = kDerivThreads * (vec ? 4 : 1);
@@ -414,39 +311,27 @@ int gated_deriv(const GatedDeriv& d) {
 #undef DERIV
   return check_launch();
 }
-int gradient_planes(const GradientPlanes& planes) {
-  GradientPlanes g = planes;
-  g.cases = planes_cases(g.H, g.N);
-  const bool vec = g.H % 4 == 0 && on16(g.gate) && on16(g.up);
-  const long blocks = deriv_grid(g.H, g.N, g.cases, vec);
-  const long extra = g.biases.part ? (2L * g.H + 31) / 32 : 0;
-  if (blocks + extra > 0x7fffffffL) return ERROR_UNSUPPORTED;
-  g.grid = (int)blocks;
-  if (vec) (void)launch_dependent(k_gradient_planes<4>, dim3((unsigned)(blocks + extra)), dim3(kDerivThreads), 0, stream(), g);
-  else (void)launch_dependent(k_gradient_planes<1>, dim3((unsigned)(blocks + extra)), dim3(kDerivThreads), 0, stream(), g);
-  return check_launch();
-}
 }  // namespace b200
 
 extern "C" {
 
-int gated_planes(cudamat* gate_w, cudamat* up_w, cudamat* gate_planes, cudamat* up_planes, cudamat* scales) {
+int gated_planes(cudamat* gate_w, cudamat* up_w, cudamat* gate_planes, cudamat* up_planes, cudamat* low_planes) {
   int err = weights_ok(gate_w, up_w);
-  if (!err) err = planes_ok(gate_w, gate_planes, up_planes, scales);
+  if (!err) err = planes_ok(gate_w, gate_planes, up_planes, low_planes);
   if (err) return err;
   const int V = gate_w->size[0], H = gate_w->size[1];
   if (V == 0 || H == 0) return 0;
-  if (overlapping({gate_planes, up_planes, scales, gate_w, up_w}, 3)) return ERROR_UNSUPPORTED;
-  const SplitJob jobs[2] = {{gate_w->data_device, (uint16_t*)gate_planes->data_device, scales->data_device, 2, H},
-                            {up_w->data_device, (uint16_t*)up_planes->data_device, scales->data_device + 1, 2, H}};
+  if (overlapping({gate_planes, up_planes, low_planes, gate_w, up_w}, 3)) return ERROR_UNSUPPORTED;
+  const SplitJob jobs[2] = {{gate_w->data_device, weight_planes(gate_w, gate_planes, low_planes, 0)},
+                            {up_w->data_device, weight_planes(up_w, up_planes, low_planes, 1)}};
   return split_columns(jobs, 2, V);
 }
 
 int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bias, cudamat* up_bias, int activation,
-                  cudamat* gate_planes, cudamat* up_planes, cudamat* scales, cudamat* gate, cudamat* up, cudamat* target) {
+                  cudamat* gate_planes, cudamat* up_planes, cudamat* low_planes, cudamat* gate, cudamat* up, cudamat* target) {
   int err = weights_ok(gate_w, up_w);
   if (err) return err;
-  if ((gate_planes || up_planes || scales) && (err = planes_ok(gate_w, gate_planes, up_planes, scales))) return err;
+  if ((gate_planes || up_planes || low_planes) && (err = planes_ok(gate_w, gate_planes, up_planes, low_planes))) return err;
   if (!mat->on_device || !target->on_device || (gate && !gate->on_device) || (up && !up->on_device)) return ERROR_NOT_ON_DEVICE;
   if (mat->is_trans || target->is_trans || (gate && gate->is_trans) || (up && up->is_trans)) return ERROR_TRANSPOSED;
   const int V = gate_w->size[0], H = gate_w->size[1], N = mat->size[1];
@@ -458,10 +343,10 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
     return ERROR_UNSUPPORTED;
   }
   if (H == 0 || N == 0) return 0;
-  if (overlapping({target, gate, up, mat, gate_w, up_w, gate_bias, up_bias, gate_planes, up_planes, scales}, 3)) return ERROR_UNSUPPORTED;
+  if (overlapping({target, gate, up, mat, gate_w, up_w, gate_bias, up_bias, gate_planes, up_planes, low_planes}, 3)) return ERROR_UNSUPPORTED;
   auto at = [](cudamat* m) { return m ? m->data_device : nullptr; };
-  // Of large layers the tensor cores read planes faster from five cases on: 2048 x 8192, 8 cases 34 us, 52 without planes (83 with the
-  // split before them), 4 cases 33 and 35.
+  // Of large layers the tensor cores read planes faster from five cases on: 2048 x 8192, 8 cases 38 us, 51 without planes (123 with the
+  // split before them), 5 cases 38 and 41, 4 cases 38 and 34.
   const bool on_groups = V % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device);
   const bool planes_first = gate_planes && N > 4 && (long)V * H >= 1L << 22;
   if (N <= kFewCases && gemm_path() == 0 && !planes_first) {
@@ -486,23 +371,16 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
   // Tensor cores, behind a launch or two that split the operands: where the products are more than those cost.
   const bool large = (long)V * H * N >= kTensorWork;
   if (V > 0 && gemm_path() != 2 && (large || gemm_path() == 1) && tma_available()) {
-    const long px = (long)aux_rows(V) * N * 4, pw = gate_planes ? 0 : (long)aux_rows(V) * H * 4;
-    const long inv = ((long)(N + 2L * H) * 4 + 255) / 256 * 256;
-    CallScratch room(6, (size_t)(px + 2 * pw + inv));
-    if (!room.p) return CUDA_ERROR;
-    uint16_t* xp = (uint16_t*)((char*)room.p + inv);
-    float* x_inv = (float*)room.p;
+    const size_t px = (planes_bytes(V, N) + 255) / 256 * 256, pw = gate_planes ? 0 : (planes_bytes(V, H) + 255) / 256 * 256;
+    CallScratch room(6, px + 2 * pw);
+    char* const p = (char*)room.p;
+    if (!p) return CUDA_ERROR;
     GatedForward f;
-    f.x = {xp, V, N};
-    f.wg = {gate_planes ? (uint16_t*)gate_planes->data_device : xp + px / 2, V, H};
-    f.wu = {gate_planes ? (uint16_t*)up_planes->data_device : xp + (px + pw) / 2, V, H};
-    float* w_inv = gate_planes ? scales->data_device : x_inv + N;
-    const SplitJob jobs[3] = {{mat->data_device, xp, x_inv, 1, N},
-                              {gate_w->data_device, (uint16_t*)f.wg.p, w_inv, 2, H},
-                              {up_w->data_device, (uint16_t*)f.wu.p, w_inv + 1, 2, H}};
+    f.x = planes_at(p, V, N);
+    f.wg = gate_planes ? weight_planes(gate_w, gate_planes, low_planes, 0) : planes_at(p + px, V, H);
+    f.wu = gate_planes ? weight_planes(up_w, up_planes, low_planes, 1) : planes_at(p + px + pw, V, H);
+    const SplitJob jobs[3] = {{mat->data_device, f.x}, {gate_w->data_device, f.wg}, {up_w->data_device, f.wu}};
     if ((err = split_columns(jobs, gate_planes ? 1 : 3, V))) return err;
-    f.w_inv = w_inv;
-    f.x_inv = x_inv;
     f.bg = at(gate_bias);
     f.bu = at(up_bias);
     f.gate = at(gate);
@@ -523,10 +401,10 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
 }
 
 int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gate_w, cudamat* up_w, cudamat* mat, int activation,
-                        cudamat* gate_planes, cudamat* up_planes, cudamat* scales, cudamat* grad_mat, cudamat* grad_gate_w, cudamat* grad_up_w, cudamat* grad_gate_bias, cudamat* grad_up_bias) {
+                        cudamat* gate_planes, cudamat* up_planes, cudamat* low_planes, cudamat* grad_mat, cudamat* grad_gate_w, cudamat* grad_up_w, cudamat* grad_gate_bias, cudamat* grad_up_bias) {
   int err = weights_ok(gate_w, up_w);
   if (err) return err;
-  if ((gate_planes || up_planes || scales) && (err = planes_ok(gate_w, gate_planes, up_planes, scales))) return err;
+  if ((gate_planes || up_planes || low_planes) && (err = planes_ok(gate_w, gate_planes, up_planes, low_planes))) return err;
   const int V = gate_w->size[0], H = gate_w->size[1], N = mat->size[1];
   struct { cudamat* m; int rows, cols; } want[] = {{deriv, H, N}, {gate, H, N}, {up, H, N}, {mat, V, N}, {grad_mat, V, N},
                                                    {grad_gate_w, V, H}, {grad_up_w, V, H}};
@@ -542,7 +420,7 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     return ERROR_UNSUPPORTED;
   }
   if (overlapping({gate, up, grad_mat, grad_gate_w, grad_up_w, grad_gate_bias, grad_up_bias, deriv, gate_w, up_w, mat, gate_planes, up_planes,
-                   scales}, 7))
+                   low_planes}, 7))
     return ERROR_UNSUPPORTED;
   if (N == 0 || H == 0) {           // sums over no cases, or no units
     for (cudamat* m : {grad_gate_bias, grad_up_bias, grad_gate_w, grad_up_w, grad_mat})
@@ -551,17 +429,16 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     return 0;
   }
   const bool biases = grad_gate_bias || grad_up_bias, weights = grad_gate_w || grad_up_w;
-  // On planes, or as four products of the matrices themselves (`dot`), which read large weights faster for few cases but take
-  // matrices that TMA cannot address behind copies.  Microseconds, planes / dot: 256 x 256, 32 cases 18 / 28; 784 x 500, 100 cases
-  // 27 / 40; 1024 x 1024, 128 cases 34 / 52; 2048 x 8192, 64 cases 167 / 149, 256 cases 209 / 233, 4096 cases 1385 / 2462; 301 x 301,
-  // 301 cases 25 / 61; 1357 x 601, 203 cases 31 / 103.
+  // On parts, or as four products of the matrices themselves (`dot`), which read large weights faster for few cases but take
+  // matrices that TMA cannot address behind copies.  Microseconds, parts / dot: 784 x 500, 100 cases 30 / 41; 1024 x 1024, 128 cases
+  // 40 / 58; 1024 x 4096, 64 cases 79 / 95; 2048 x 8192, 64 cases 196 / 149, 4096 cases 2491 / 2849.
   const bool aligned = V % 4 == 0 && H % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device) &&
                        on16(gate->data_device) && on16(up->data_device);
   const bool few = aligned && !gate_planes && N < 128 && (long)V * H >= 1L << 22;
   const bool large = (long)V * H * N >= 1L << 16 && !few;
   const bool tc = V > 0 && (weights || grad_mat) && gemm_path() != 2 && (large || gemm_path() == 1) && tma_available();
   const int cases = gated_deriv_cases(N), blocks = (N + cases - 1) / cases;
-  const bool split_w = tc && !gate_planes;
+  const bool split_w = tc && grad_mat && !gate_planes;
   // scratch, each part on 256 bytes
   size_t room_bytes = 0;
   auto take = [&](bool wanted, size_t bytes) {
@@ -569,11 +446,9 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     if (wanted) room_bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  const size_t unit = sizeof(float) * 2 * (size_t)H, each = sizeof(float) * (size_t)N, hn = (size_t)aux_rows(H) * N * 4;
-  const size_t at_part = take(biases, unit * blocks), at_tmax = take(tc, each), at_umax = take(tc, unit), after_max = room_bytes;
-  const size_t at_xi = take(tc, each), at_wi = take(split_w, unit), at_ci = take(tc, each), at_ui = take(tc, unit);
-  const size_t at_x = take(tc, (size_t)aux_rows(V) * N * 4), vh = (size_t)aux_rows(V) * H * 4, at_wg = take(split_w, vh), at_wu = take(split_w, vh);
-  const size_t at_cg = take(tc && grad_mat, hn), at_cu = take(tc && grad_mat, hn), at_ug = take(tc && weights, hn), at_uu = take(tc && weights, hn);
+  const size_t at_part = take(biases, sizeof(float) * 2 * (size_t)H * blocks), at_x = take(tc && weights, planes_bytes(V, N));
+  const size_t at_wg = take(split_w, planes_bytes(V, H)), at_wu = take(split_w, planes_bytes(V, H));
+  const size_t at_g = take(tc, planes_bytes(H, N)), at_u = take(tc, planes_bytes(H, N));
   CallScratch room(6, room_bytes);
   char* const p = (char*)room.p;
   if (room_bytes && !p) return CUDA_ERROR;
@@ -588,23 +463,24 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
   d.part = biases ? (float*)(p + at_part) : nullptr;
   Planes xp = {}, wgp = {}, wup = {};
   if (tc) {
-    d.token_max = (uint32_t*)(p + at_tmax);
-    d.unit_max = (uint32_t*)(p + at_umax);
-    d.x_inv = (float*)(p + at_xi);
-    d.w_inv = split_w ? (float*)(p + at_wi) : scales->data_device;
-    xp = {(uint16_t*)(p + at_x), V, N};
-    wgp = {split_w ? (uint16_t*)(p + at_wg) : (uint16_t*)gate_planes->data_device, V, H};
-    wup = {split_w ? (uint16_t*)(p + at_wu) : (uint16_t*)up_planes->data_device, V, H};
-    const SplitJob jobs[3] = {{mat->data_device, (uint16_t*)xp.p, (float*)d.x_inv, 1, N},
-                              {gate_w->data_device, (uint16_t*)wgp.p, (float*)d.w_inv, 2, H},
-                              {up_w->data_device, (uint16_t*)wup.p, (float*)d.w_inv + 1, 2, H}};
-    if ((err = split_columns(jobs, split_w ? 3 : 1, V, d.token_max, (int)((after_max - at_tmax) / 4)))) return err;
+    SplitJob jobs[3];
+    int njobs = 0;
+    if (weights) jobs[njobs++] = {mat->data_device, xp = planes_at(p + at_x, V, N)};
+    if (split_w) {
+      jobs[njobs++] = {gate_w->data_device, wgp = planes_at(p + at_wg, V, H)};
+      jobs[njobs++] = {up_w->data_device, wup = planes_at(p + at_wu, V, H)};
+    } else if (grad_mat) {
+      wgp = weight_planes(gate_w, gate_planes, low_planes, 0);
+      wup = weight_planes(up_w, up_planes, low_planes, 1);
+    }
+    if (njobs && (err = split_columns(jobs, njobs, V))) return err;
+    d.parts_g = planes_at(p + at_g, H, N);
+    d.parts_u = planes_at(p + at_u, H, N);
   }
   if ((err = gated_deriv(d))) return err;
-  const BiasSums sums = {d.part, blocks, H, grad_gate_bias ? grad_gate_bias->data_device : nullptr,
-                         grad_up_bias ? grad_up_bias->data_device : nullptr};
-  if (biases && !tc) {
-    (void)launch_dependent(k_gated_biases, dim3((2 * (unsigned)H + 31) / 32), dim3(kDerivThreads), 0, stream(), sums);
+  if (biases) {
+    (void)launch_dependent(k_gated_biases, dim3((2 * (unsigned)H + 31) / 32), dim3(kDerivThreads), 0, stream(), d.part, blocks, H,
+                           grad_gate_bias ? grad_gate_bias->data_device : nullptr, grad_up_bias ? grad_up_bias->data_device : nullptr);
     if ((err = check_launch())) return err;
   }
   if (!tc) {
@@ -619,27 +495,6 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     }
     return 0;
   }
-  GradientPlanes g = {};
-  if (biases) g.biases = sums;
-  g.gate = d.gate;
-  g.up = d.up;
-  g.H = H;
-  g.N = N;
-  g.w_inv = d.w_inv;
-  g.x_inv = d.x_inv;
-  g.token_max = d.token_max;
-  g.unit_max = d.unit_max;
-  g.case_inv = (float*)(p + at_ci);
-  g.unit_inv = (float*)(p + at_ui);
-  if (grad_mat) {
-    g.by_case[0] = (uint16_t*)(p + at_cg);
-    g.by_case[1] = (uint16_t*)(p + at_cu);
-  }
-  if (weights) {
-    g.by_unit[0] = (uint16_t*)(p + at_ug);
-    g.by_unit[1] = (uint16_t*)(p + at_uu);
-  }
-  if ((err = gradient_planes(g))) return err;
   PlaneProduct f[2] = {};
   int products = 0;
   if (grad_mat) {
@@ -647,25 +502,21 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     x.npairs = 2;
     x.a[0] = wgp;
     x.a[1] = wup;
-    x.b[0] = {g.by_case[0], H, N};
-    x.b[1] = {g.by_case[1], H, N};
+    x.b[0] = d.parts_g;
+    x.b[1] = d.parts_u;
     x.nout = 1;
     x.out[0] = grad_mat->data_device;
-    x.inv[0] = g.case_inv;
-    x.inv_stride = 1;
   }
   if (weights) {
     PlaneProduct& w = f[products++];
     w.npairs = 1;
     w.trans = true;
     w.a[0] = xp;
-    w.inv_stride = 2;
     cudamat* const out[2] = {grad_gate_w, grad_up_w};
     for (int k = 0; k < 2; k++) {
       if (!out[k]) continue;
-      w.b[w.nout] = {g.by_unit[k], H, N};
-      w.out[w.nout] = out[k]->data_device;
-      w.inv[w.nout++] = g.unit_inv + k;
+      w.b[w.nout] = k ? d.parts_u : d.parts_g;
+      w.out[w.nout++] = out[k]->data_device;
     }
   }
   return plane_products(f, products);

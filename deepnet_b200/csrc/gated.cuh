@@ -1,4 +1,4 @@
-// Products of a gated layer on scaled half-precision planes (gated_tc.cu), as gated.cu calls them.
+// Products of a gated layer on bfloat16 parts (gated_tc.cu), as gated.cu calls them.
 #pragma once
 #include "common.cuh"
 
@@ -27,79 +27,104 @@ __device__ __forceinline__ float activate(float g, float& slope) {
   slope = 1.0f;
   return g;
 }
+
+// kVec consecutive floats (4: the address is on 16 bytes).
+template <int kVec>
+__device__ __forceinline__ void load(const float* p, float (&v)[kVec]) {
+  if constexpr (kVec == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  } else {
+    v[0] = *p;
+  }
+}
+template <int kVec>
+__device__ __forceinline__ void store(float* p, const float (&v)[kVec]) {
+  if constexpr (kVec == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else *p = v[0];
+}
+
+// x = hi + mid + lo, each the bfloat16 nearest to what is left (hi the largest finite one at most): 24 bits in three times eight, exact
+// from magnitudes of 2^-103 on (below, lo is no normal number).  Infinities and NaN are in hi alone.
+__device__ __forceinline__ void split_parts(float x, uint16_t& lo, uint16_t& mid, uint16_t& hi) {
+  const bool finite = fabsf(x) <= 3.4028234e38f;
+  hi = float_to_bf16(x);
+  if (finite && (hi & 0x7fffu) == 0x7f80u) hi -= 1;
+  const float rest = finite ? x - bf16_to_float(hi) : 0.0f;
+  mid = float_to_bf16(rest);
+  lo = float_to_bf16(rest - bf16_to_float(mid));
+}
 #endif
 
-// A rows x cols matrix as planes, in an aux matrix's layout (common.cuh): column c times 2^e(c), split into two half-precision
-// numbers; inv[c * inv_stride] = 2^-e(c).  e puts the column's largest finite magnitude into (2^12, 2^13].
+// A rows x cols matrix as three bfloat16 parts of its elements.  p: mid and hi, in an aux matrix's layout (common.cuh; plane 0, 1);
+// low: columns of lo, low_ld apart (a multiple of 8).
 struct Planes {
-  const uint16_t* p;
-  int rows, cols;
-  long bytes() const { return (long)aux_rows(rows) * cols * 4; }
+  uint16_t *p, *low;
+  int low_ld, rows, cols;
 };
+inline size_t planes_bytes(int rows, int cols) { return (size_t)aux_rows(rows) * cols * 6; }
+inline Planes planes_at(void* at, int rows, int cols) {          // on 16 bytes
+  uint16_t* p = (uint16_t*)at;
+  return {p, p + (size_t)2 * aux_rows(rows) * cols, aux_rows(rows), rows, cols};
+}
 struct SplitJob {
   const float* x;
-  uint16_t* planes;
-  float* inv;
-  int inv_stride, cols;
+  Planes to;
 };
-// Up to three matrices of the same number of rows, in one launch, which sets nzero words to zero too.
-int split_columns(const SplitJob* jobs, int njobs, int rows, uint32_t* zero = nullptr, int nzero = 0);
+// Up to three matrices of the same number of rows, in one launch.
+int split_columns(const SplitJob* jobs, int njobs, int rows);
 
-// y = act(Wg' x + bg) * (Wu' x + bu); w_inv: 2 x H, gate's and up's
+#ifdef __CUDACC__
+// Elements r .. of column c (kVec 4: r is a multiple of 4).
+template <int kVec>
+__device__ __forceinline__ void store_parts(const Planes& to, int r, long c, const float (&v)[kVec]) {
+  const int lda = aux_rows(to.rows);
+  uint16_t l[kVec], m[kVec], h[kVec], *at = to.p + c * 2 * lda + r, *low = to.low + c * to.low_ld + r;
+#pragma unroll
+  for (int j = 0; j < kVec; j++) split_parts(v[j], l[j], m[j], h[j]);
+  if constexpr (kVec == 4) {
+    *reinterpret_cast<ushort4*>(low) = make_ushort4(l[0], l[1], l[2], l[3]);
+    *reinterpret_cast<ushort4*>(at) = make_ushort4(m[0], m[1], m[2], m[3]);
+    *reinterpret_cast<ushort4*>(at + lda) = make_ushort4(h[0], h[1], h[2], h[3]);
+  } else {
+    low[0] = l[0];
+    at[0] = m[0];
+    at[lda] = h[0];
+  }
+}
+#endif
+
+// y = act(Wg' x + bg) * (Wu' x + bu)
 struct GatedForward {
   Planes wg, wu, x;
-  const float *w_inv, *x_inv, *bg, *bu;
+  const float *bg, *bu;
   float *gate, *up, *y;
   int activation;
 };
 int gated_tc(const GatedForward& f);
 
-// out[:, n] = inv(n) sum over the pairs (a, b) of a . op(b): planes of a as stored (their rows are the output's), of b as stored
-// (its columns are the output's, `trans` false, up to two pairs) or transposed (its rows are; one pair, and with a second b a second
-// out, for the same a).
+// out = sum over the pairs (a, b) of a . op(b): a as stored (its rows are the output's), b as stored (its columns are the output's, `trans`
+// false, up to two pairs) or transposed (its rows are; one pair, and with a second b a second out, for the same a).
 struct PlaneProduct {
   int npairs;
   Planes a[2], b[2];
   bool trans;
   int nout;
   float* out[2];
-  const float* inv[2];      // of out's columns; stride inv_stride
-  int inv_stride;
 };
 int plane_products(const PlaneProduct* f, int nproducts);      // one or two, in one launch
 
-// gate, up = their gradients dG, dU from dy; with `maxima` the largest |dG| w_inv, |dU| w_inv of each case (token_max) and the largest
-// |dG| x_inv, |dU| x_inv of each unit (unit_max, gate's and up's): bits of floats, all zero before.  part: sums of dG and dU over the
-// cases of a block, blocks of `cases` x 2 x H, or null.
+// gate, up = their gradients dG, dU from dy; with parts_g.p these as parts too.  part: sums of dG and dU over the cases of a block, blocks
+// of `cases` x 2 x H, or null.
 struct GatedDeriv {
   const float* dy;
   float *gate, *up;
   int H, N, activation;
-  const float *w_inv, *x_inv;
-  uint32_t *token_max, *unit_max;
+  Planes parts_g, parts_u;
   float* part;
   int cases;                // of a block
 };
 int gated_deriv_cases(int N);
 int gated_deriv(const GatedDeriv& d);
-// Sums over the blocks of `part` (GatedDeriv): of dG and dU over all cases.
-struct BiasSums {
-  const float* part;
-  int blocks, H;
-  float *gate, *up;
-};
-// dG and dU as planes: with the weights' scales divided out and one of their own a case (by_case: gate's, up's; inverses case_inv),
-// and with the inputs' scales divided out and one of their own a unit (by_unit; unit_inv 2 x H).  Either may be null.
-struct GradientPlanes {
-  const float *gate, *up;
-  int H, N;
-  const float *w_inv, *x_inv;
-  const uint32_t *token_max, *unit_max;
-  uint16_t *by_case[2], *by_unit[2];
-  float *case_inv, *unit_inv;
-  int cases, grid;          // set by the call
-  BiasSums biases;          // part not null: summed by the same launch
-};
-int gradient_planes(const GradientPlanes& g);
 
 }  // namespace b200

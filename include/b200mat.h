@@ -302,18 +302,20 @@ int layer_norm_deriv(cudamat* deriv, cudamat* mat, cudamat* stats, cudamat* gain
 
 /* A gated layer: target (H x N) = act(gate_w' mat + gate_bias) * (up_w' mat + up_bias), weights V x H, mat V x N, biases (one value a
  * unit) or null; activation 0 none, 1 logistic, 2 max(0, g), 3 g logistic(g), 4 g Phi(g).  gate and up (H x N, both or neither) receive
- * the sums the activation is taken of, for the derivative.  No result of this call or the next may lie over another argument. */
+ * the sums the activation is taken of, for the derivative.  No result of this call or the next may lie over another argument.
+ * Products are of float32 grade at every size, each held to its own terms; operands below 2^-103 keep fewer bits on the tensor cores.
+ * An infinite weight or input makes its unit's or its case's results infinite or NaN, which of the two goes by the kernel. */
 int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bias, cudamat* up_bias, int activation,
-                  cudamat* gate_planes, cudamat* up_planes, cudamat* scales, cudamat* gate, cudamat* up, cudamat* target);
-/* The weights' form for the tensor cores, for layers that run many times between changes of their weights: gate_planes, up_planes
- * (aux handles of the weights, on 16 bytes) receive every column times a power of two as two half-precision planes, scales (2 x H) the
- * powers' inverses.  gated_product takes all three (or none: it splits the weights itself) and reads them instead of the weights where
- * tensor cores run; they have to be filled again when the weights change. */
-int gated_planes(cudamat* gate_w, cudamat* up_w, cudamat* gate_planes, cudamat* up_planes, cudamat* scales);
+                  cudamat* gate_planes, cudamat* up_planes, cudamat* low_planes, cudamat* gate, cudamat* up, cudamat* target);
+/* The weights' form for the tensor cores, for layers that run many times between changes of their weights: gate_planes, up_planes and
+ * low_planes (aux handles of the weights, on 16 bytes) receive three bfloat16 numbers for every weight that add up to it (the smallest
+ * of both in low_planes).  gated_product takes all three (or none: it splits the weights itself) and reads them instead of the weights
+ * where tensor cores run; they have to be filled again when the weights change. */
+int gated_planes(cudamat* gate_w, cudamat* up_w, cudamat* gate_planes, cudamat* up_planes, cudamat* low_planes);
 /* deriv: the gradient of gated_product's target.  gate and up, as it left them, are overwritten with their gradients; the others
  * receive those of mat, weights and biases (null: not wanted), summed in a fixed order.  Planes as in gated_product. */
 int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gate_w, cudamat* up_w, cudamat* mat, int activation,
-                        cudamat* gate_planes, cudamat* up_planes, cudamat* scales, cudamat* grad_mat, cudamat* grad_gate_w,
+                        cudamat* gate_planes, cudamat* up_planes, cudamat* low_planes, cudamat* grad_mat, cudamat* grad_gate_w,
                         cudamat* grad_up_w, cudamat* grad_gate_bias, cudamat* grad_up_bias);
 
 /* target = add + (u > dropprob ? mat / (1 - dropprob) : 0), add (or null: 0) of mat's shape, u the uniforms that fill_with_rand would

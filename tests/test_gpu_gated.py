@@ -395,3 +395,103 @@ def test_results_of_more_than_2_to_31_elements(cm):
     assert (get(y.slice(0, 2)) == 0).all()
     y.free_device_memory()
     assert cm.read_status() == 0
+
+
+def by_terms(a, b):
+    """How far a . b may be off by its own terms alone, whatever else a row or column holds: operands are exact sums of three parts
+    of eight bits, products of parts below 2^-26 of |a_k||b_k| are left out, a sum of 64 terms lies in the tensor core for four
+    instructions at its full size and twenty at 2^-8 of it, each of which drops up to 2^-22 of it (4.2 x 2^-22), and the sums of 64
+    are added in float32; full float32 multiply-adds round K times.  2^-19 + (K + 2) u covers either."""
+    return ((a.shape[1] + 2) * U + 2.0 ** -19) * (np.abs(a) @ np.abs(b))
+
+
+def gradients(cm, path, dy, gate, up, wg, wu, x):
+    """dg, du, dx, dwg, dwu of the layer with relu."""
+    G = cm.CUDAMatrix
+    gm, um = G(gate), G(up)
+    out = [cm.empty(s) for s in (x.shape, wg.shape, wu.shape)]
+    on_path(cm, path, lambda: cm.gated_product_deriv(G(dy), gm, um, G(wg), G(wu), G(x), activation="relu", grad_x=out[0],
+                                                     grad_gate_w=out[1], grad_up_w=out[2]))
+    return [get(m) for m in [gm, um] + out]
+
+
+def check_both_ways(cm, path, wg, wu, x, gate, up, dy, least=1e-36):
+    V, H = wg.shape
+    N = x.shape[1]
+    gm, um = cm.empty((H, N)), cm.empty((H, N))
+    G = cm.CUDAMatrix
+    on_path(cm, path, lambda: cm.gated_product(G(wg), G(wu), G(x), activation="linear", gate=gm, up=um))
+    A, B, X = (v.astype(np.float64) for v in (wg, wu, x))
+    within(get(gm), A.T @ X, by_terms(A.T, X) + least)
+    within(get(um), B.T @ X, by_terms(B.T, X) + least)
+    dg, du, dx, dwg, dwu = gradients(cm, path, dy, gate, up, wg, wu, x)
+    assert np.array_equal(dg, dy * up * (gate > 0)) and np.array_equal(du, dy * np.maximum(gate, 0))
+    D, E = dg.astype(np.float64), du.astype(np.float64)
+    AB, DE = np.concatenate([A, B], 1), np.concatenate([D, E], 0)
+    within(dx, AB @ DE, by_terms(AB, DE) + least)
+    within(dwg, X @ D.T, by_terms(X, D.T) + least)
+    within(dwu, X @ E.T, by_terms(X, E.T) + least)
+    assert cm.read_status() == 0
+
+
+SPREAD_SHAPES = [(784, 64, 64), (300, 200, 40), (257, 129, 130), (2048, 256, 33)]
+
+
+@pytest.mark.parametrize("path", [0, 1, 2])
+@pytest.mark.parametrize("spread", [0, 13, 20, 27, 40, 50])
+@pytest.mark.parametrize("shape", SPREAD_SHAPES)
+def test_small_entries_beside_large_ones_of_their_column(cm, shape, spread, path):
+    """A feature 2^spread above the others whose weights are as far below theirs, features all over that range, and the same of the
+    units' gradients: every sum is held to its own terms."""
+    V, H, N = shape
+    rng = np.random.default_rng(V + H + N + spread)
+    normal = lambda *s: rng.standard_normal(s)
+    e = rng.integers(-spread // 2, spread // 2 + 1, (V, 1))
+    e[:4] = spread
+    e[4:V // 2] = 0
+    wg, wu = (np.ldexp(normal(V, H), -e).astype(np.float32) for _ in range(2))
+    x = np.ldexp(normal(V, N), e).astype(np.float32)
+    f = rng.integers(-spread // 2, spread // 2 + 1, (H, 1))
+    f[:3], f[3:H // 2] = spread, 0
+    c = rng.integers(-8, 9, (1, N))               # (2^50 2^50 2^8 and what the sums add: every result is a normal number)
+    dy = np.ldexp(normal(H, N), f + c).astype(np.float32)
+    check_both_ways(cm, path, wg, wu, x, normal(H, N).astype(np.float32), normal(H, N).astype(np.float32), dy)
+
+
+@pytest.mark.parametrize("path", [0, 1, 2])
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-6, 1e-8, 1e-12])
+def test_a_unit_and_a_case_of_zeros_cost_the_others_nothing(cm, size, path):
+    rng = np.random.default_rng(5)
+    V, H, N = 300, 200, 64
+    normal = lambda *s: rng.standard_normal(s).astype(np.float32)
+    wg, wu, x = (size * normal(*s) for s in ((V, H), (V, H), (V, N)))
+    wg[:, 7] = 0
+    wu[:, [7, 11]] = 0
+    x[:, 9] = 0
+    check_both_ways(cm, path, wg, wu, x, np.abs(normal(H, N)), normal(H, N), normal(H, N))
+
+
+@pytest.mark.parametrize("path", [0, 1, 2])
+@pytest.mark.parametrize("ends", [(120, -100, -20), (-100, 20, 90), (124, -90, -40), (-90, 100, -80), (60, 60, -60), (100, -100, -100)])
+def test_magnitudes_at_both_ends_of_the_range(cm, ends, path):
+    """Weights, inputs and gradients about 2^ends: no power of two is out of reach where the result is a normal number."""
+    rng = np.random.default_rng(6)
+    V, H, N = 200, 140, 40
+    normal = lambda *s: rng.standard_normal(s)
+    wg, wu, x, dy = (np.ldexp(normal(*s), e).astype(np.float32) for s, e in zip(((V, H), (V, H), (V, N), (H, N)), (ends[0],) + ends))
+    check_both_ways(cm, path, wg, wu, x, np.abs(normal(H, N)).astype(np.float32), normal(H, N).astype(np.float32), dy, least=2.0 ** -118)
+
+
+def test_the_largest_number_there_is(cm):
+    """It is above the largest of eight bits: its parts still add up to it."""
+    V, H, N = 300, 128, 64
+    top = np.finfo(np.float32).max
+    x = np.zeros((V, N), np.float32)
+    x[np.arange(N), np.arange(N)] = top
+    x[np.arange(N), (np.arange(N) + 1) % N] = -top
+    w = np.ldexp(np.random.default_rng(7).standard_normal((V, H)), -20).astype(np.float32)
+    gm, um = cm.empty((H, N)), cm.empty((H, N))
+    on_path(cm, 1, lambda: cm.gated_product(cm.CUDAMatrix(w), cm.CUDAMatrix(-w), cm.CUDAMatrix(x), activation="linear", gate=gm, up=um))
+    A, X = w.astype(np.float64), x.astype(np.float64)
+    within(get(gm), A.T @ X, by_terms(A.T, X))
+    assert np.array_equal(get(um), -get(gm))
