@@ -519,7 +519,7 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
       w.out[w.nout++] = out[k]->data_device;
     }
   }
-  return plane_products(f, products);
+  return plane_products(f, products, V, H, N);
 }
 
 }  // extern "C"

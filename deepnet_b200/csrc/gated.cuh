@@ -28,12 +28,15 @@ __device__ __forceinline__ float activate(float g, float& slope) {
   return g;
 }
 
-// kVec consecutive floats (4: the address is on 16 bytes).
+// kVec consecutive floats (4, 8: the address is on 16 bytes).
 template <int kVec>
 __device__ __forceinline__ void load(const float* p, float (&v)[kVec]) {
-  if constexpr (kVec == 4) {
-    const float4 x = *reinterpret_cast<const float4*>(p);
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  if constexpr (kVec % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < kVec; j += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p + j);
+      v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
+    }
   } else {
     v[0] = *p;
   }
@@ -44,15 +47,19 @@ __device__ __forceinline__ void store(float* p, const float (&v)[kVec]) {
   else *p = v[0];
 }
 
-// x = hi + mid + lo, each the bfloat16 nearest to what is left (hi the largest finite one at most): 24 bits in three times eight, exact
-// from magnitudes of 2^-103 on (below, lo is no normal number).  Infinities and NaN are in hi alone.
-__device__ __forceinline__ void split_parts(float x, uint16_t& lo, uint16_t& mid, uint16_t& hi) {
-  const bool finite = fabsf(x) <= 3.4028234e38f;
-  hi = float_to_bf16(x);
-  if (finite && (hi & 0x7fffu) == 0x7f80u) hi -= 1;
-  const float rest = finite ? x - bf16_to_float(hi) : 0.0f;
-  mid = float_to_bf16(rest);
-  lo = float_to_bf16(rest - bf16_to_float(mid));
+// x = hi + mid + lo, each the bfloat16 (a float's upper half) nearest to what is left, hi the largest finite one at most: 24 bits in
+// three times eight, exact from magnitudes of 2^-103 on (below, lo is no normal number).  Infinities and NaN are in hi alone.
+__device__ __forceinline__ void split_parts(float x, uint32_t& lo, uint32_t& mid, uint32_t& hi) {
+  const uint32_t u = __float_as_uint(x);
+  hi = (u + 0x8000u) & 0xffff0000u;
+  float rest = x - __uint_as_float(hi);
+  if ((u & 0x7fffffffu) >= 0x7f7f8000u) {            // would round to infinity, is infinite, or NaN
+    const bool finite = fabsf(x) <= 3.4028234e38f;
+    hi = finite || x == x ? u & 0xffff0000u : 0x7fff0000u;
+    rest = finite ? x - __uint_as_float(hi) : 0.0f;
+  }
+  mid = (__float_as_uint(rest) + 0x8000u) & 0xffff0000u;
+  lo = __float_as_uint(rest - __uint_as_float(mid));
 }
 #endif
 
@@ -75,22 +82,28 @@ struct SplitJob {
 int split_columns(const SplitJob* jobs, int njobs, int rows);
 
 #ifdef __CUDACC__
-// Elements r .. of column c (kVec 4: r is a multiple of 4).
+// Elements r .. of column c (kVec 4, 8: r is a multiple of it).
 template <int kVec>
 __device__ __forceinline__ void store_parts(const Planes& to, int r, long c, const float (&v)[kVec]) {
   const int lda = aux_rows(to.rows);
-  uint16_t l[kVec], m[kVec], h[kVec], *at = to.p + c * 2 * lda + r, *low = to.low + c * to.low_ld + r;
+  uint32_t l[kVec], m[kVec], h[kVec];
+  uint16_t *at = to.p + c * 2 * lda + r, *low = to.low + c * to.low_ld + r;
 #pragma unroll
   for (int j = 0; j < kVec; j++) split_parts(v[j], l[j], m[j], h[j]);
-  if constexpr (kVec == 4) {
-    *reinterpret_cast<ushort4*>(low) = make_ushort4(l[0], l[1], l[2], l[3]);
-    *reinterpret_cast<ushort4*>(at) = make_ushort4(m[0], m[1], m[2], m[3]);
-    *reinterpret_cast<ushort4*>(at + lda) = make_ushort4(h[0], h[1], h[2], h[3]);
-  } else {
-    low[0] = l[0];
-    at[0] = m[0];
-    at[lda] = h[0];
-  }
+  auto put = [](uint16_t* p, const uint32_t (&x)[kVec]) {
+    if constexpr (kVec == 1) {
+      *p = (uint16_t)(x[0] >> 16);
+    } else {
+      uint32_t two[kVec / 2];                          // upper halves, side by side
+#pragma unroll
+      for (int j = 0; j < kVec; j += 2) two[j / 2] = __byte_perm(x[j], x[j + 1], 0x7632);
+      if constexpr (kVec == 8) *reinterpret_cast<uint4*>(p) = make_uint4(two[0], two[1], two[2], two[3]);
+      else *reinterpret_cast<uint2*>(p) = make_uint2(two[0], two[1]);
+    }
+  };
+  put(low, l);
+  put(at, m);
+  put(at + lda, h);
 }
 #endif
 
@@ -112,7 +125,8 @@ struct PlaneProduct {
   int nout;
   float* out[2];
 };
-int plane_products(const PlaneProduct* f, int nproducts);      // one or two, in one launch
+// One or two in one launch: the inputs' gradient (two pairs) and the weights' (transposed), of a layer of V inputs and H units.
+int plane_products(const PlaneProduct* f, int nproducts, int V, int H, int cases);
 
 // gate, up = their gradients dG, dU from dy; with parts_g.p these as parts too.  part: sums of dG and dU over the cases of a block, blocks
 // of `cases` x 2 x H, or null.

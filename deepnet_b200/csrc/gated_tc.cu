@@ -13,7 +13,7 @@
 // both operands, 64 products deep, and is free again behind its last instruction, so that two stages of 256 columns are enough.  The
 // accumulator truncates at every instruction, so sums are folded into registers every 64 products (two buffers in tensor memory), the
 // small products first.  Every wait is bounded; on expiry the kernel records a status word, drains and returns.  2048 x 8192,
-// 4096 cases: 1049 us, 262 TFLOP/s (six terms: 1573 of the tensor pipe's).
+// 4096 cases: 1030 us, 267 TFLOP/s (six terms: 1600 of the tensor pipe's).
 #include <cuda.h>
 
 #include "gated.cuh"
@@ -555,10 +555,11 @@ struct SplitJobs {
   int h;
 };
 
-// A warp a column, or a part of it (grid.y): kBatch groups of kVec values a lane on their way.  Bound by HBM: 10 bytes a value.
+// A warp a column, or a part of it (grid.y): kBatch groups of kVec values a lane on their way.  Bound by HBM: 10 bytes a value;
+// two matrices of 2048 x 8192 53 us, 6.3 TB/s (79 with four values a lane and conversions in place of integer rounding).
 template <int kVec>
 __global__ void __launch_bounds__(256) k_split_columns(const __grid_constant__ SplitJobs a) {
-  constexpr int kBatch = kVec == 4 ? 4 : 8;
+  constexpr int kBatch = kVec == 8 ? 2 : kVec == 4 ? 4 : 8;
   grid_dependents_launch();
   grid_dependency_wait();
   const int which = blockIdx.x >= a.first[2] ? 2 : blockIdx.x >= a.first[1] ? 1 : 0;
@@ -594,10 +595,12 @@ int split_columns(const SplitJob* jobs, int njobs, int rows) {
     at += (jobs[i].to.cols + 7) / 8;
   }
   if (at == 0) return 0;
+  const bool eights = vec && rows % 8 == 0;
   const int per = 32 * (vec ? 16 : 8);                   // rows of a warp's batch
   int parts = (rows + per - 1) / per;
   if (parts > 65535) parts = 65535;
-  if (vec) (void)launch_dependent(k_split_columns<4>, dim3(at, parts), dim3(256), 0, stream(), a);
+  if (eights) (void)launch_dependent(k_split_columns<8>, dim3(at, parts), dim3(256), 0, stream(), a);
+  else if (vec) (void)launch_dependent(k_split_columns<4>, dim3(at, parts), dim3(256), 0, stream(), a);
   else (void)launch_dependent(k_split_columns<1>, dim3(at, parts), dim3(256), 0, stream(), a);
   return check_launch();
 }
@@ -627,20 +630,20 @@ int gated_tc(const GatedForward& f) {
   p.spin_limit = wait_limit();
   p.tiles_m = (p.M + 127) / 128;
   // The tile's width, and whether the sums are shared out: what the pairs of CTAs need for their share of the work, in cycles.  A
-  // stage takes as long as its instructions (12 BN) or the rows its copies bring (5.4 each); sums that are shared out cost a launch
-  // and their way through memory.
+  // stage takes as long as its instructions (12 BN) or the rows its copies bring; sums that are shared out cost a launch and their way
+  // through memory.  Constants fitted to 20 shapes from 64 x 64 x 2000 to 2048 x 8192 x 1024 at every width and split: what it chooses
+  // takes 2 % longer than the best of them on average, 13 % at most (4096 x 512, 20 cases: 17.6 us, 15.5).
   const long pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, stages = (p.K + kK - 1) / kK;
   int bn = 256;
   double best = 0;
   for (int w = 256; w >= 32; w /= 2) {
     const long tiles = (long)p.tiles_m * ((p.N + w - 1) / w);
-    for (long s = 1; s <= 16 && s * 2 <= (stages > 2 ? stages : 2); s++) {
+    for (long s = 1; s <= 16 && s <= stages; s++) {
       const long turns = (tiles * s + pairs - 1) / pairs;
       if (s > 1 && turns > 1) break;
-      const double stage = 12.0 * w > 5.4 * (256 + w) ? 12.0 * w : 5.4 * (256 + w);
-      const double cost = turns * (stage * ((stages + s - 1) / s) + 2500.0 + 10.0 * w) +
-                          (s > 1 ? 12000.0 + (double)s * p.M * p.N * 8.0 / 1500.0 : 0.0);
-      if (best == 0 || cost < 0.97 * best) {
+      const double stage = 12.0 * w > 3.6 * (256 + w) ? 12.0 * w : 3.6 * (256 + w);
+      const double cost = turns * (stage * ((stages + s - 1) / s) + 400.0 + 13.0 * w) + (s > 1 ? 3500.0 + (double)s * p.M * p.N / 240.0 : 0.0);
+      if (best == 0 || cost < best) {
         best = cost;
         bn = w;
         p.splits = (int)s;
@@ -672,23 +675,43 @@ int gated_tc(const GatedForward& f) {
   return check_launch();
 }
 
-int plane_products(const PlaneProduct* f, int nproducts) {
+int plane_products(const PlaneProduct* f, int nproducts, int V, int H, int cases) {
   ProductParams p = {};
   p.status = status_word();
   p.spin_limit = wait_limit();
   const long pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
-  // The wider tile reads less shared memory a multiply-add; the narrower one where it needs fewer turns of the pairs.  Work counted in
-  // stages of a tile.
-  auto stages = [&](int w) {
-    long n = 0;
-    for (int i = 0; i < nproducts; i++) {
-      const long N = f[i].trans ? f[i].b[0].rows : f[i].b[0].cols;
-      n += (long)((f[i].a[0].rows + 255) / 256) * f[i].nout * ((N + w - 1) / w) * f[i].npairs * ((f[i].a[0].cols + kK - 1) / kK);
+  // The tile's width and how many each product's sums are shared out to (a pair of CTAs walks the items pairs apart, the inputs' gradient
+  // first): what the pair with most work needs, in cycles, as in gated_tc.  As if all gradients were wanted, so that none's bits depend on
+  // the others.  Fitted to the same 20 shapes: 3 % above the best on average, 30 % at most (128 x 2000, 150 cases: 33 us, 26).
+  int bn = 256, splits[2] = {1, 1};
+  double best = 0;
+  for (int w = 256; w >= 128; w /= 2) {
+    const double stage = 12.0 * w > 4.2 * (256 + w) ? 12.0 * w : 4.2 * (256 + w);
+    const long tiles[2] = {(V + 255) / 256 * (((long)cases + w - 1) / w), (V + 255) / 256 * (((long)H + w - 1) / w) * 2};
+    const long all[2] = {2 * (((long)H + kK - 1) / kK), ((long)cases + kK - 1) / kK}, size[2] = {(long)V * cases, 2L * V * H};
+    constexpr int kChoices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24};
+    for (int s0 : kChoices) {
+      if (s0 > all[0]) break;
+      for (int s1 : kChoices) {
+        if (s1 > all[1]) break;
+        const long n = tiles[0] * s0, total = n + tiles[1] * s1;
+        const double l0 = stage * ((all[0] + s0 - 1) / s0) + 17.0 * w, l1 = stage * ((all[1] + s1 - 1) / s1) + 17.0 * w;
+        double cost = 0;
+        for (long i : {0L, n % pairs, total % pairs}) {       // (pairs between these have the same items)
+          const long c0 = n / pairs + (i < n % pairs), c = total / pairs + (i < total % pairs);
+          const double t = c0 * l0 + (c - c0) * l1;
+          if (t > cost) cost = t;
+        }
+        if (s0 > 1 || s1 > 1) cost += 4200.0 + ((s0 > 1 ? (double)s0 * size[0] : 0.0) + (s1 > 1 ? (double)s1 * size[1] : 0.0)) / 300.0;
+        if (best == 0 || cost < best) {
+          best = cost;
+          bn = w;
+          splits[0] = s0;
+          splits[1] = s1;
+        }
+      }
     }
-    return n;
-  };
-  const int bn = 2 * ((stages(256) + pairs - 1) / pairs) <= 1.1 * ((stages(128) + pairs - 1) / pairs) ? 256 : 128;
-  const long share = (stages(bn) + pairs - 1) / pairs;       // stages a pair has to do at least
+  }
   size_t bytes = 0;
   long items = 0;
   for (int i = 0; i < nproducts; i++) {
@@ -701,11 +724,7 @@ int plane_products(const PlaneProduct* f, int nproducts) {
     q.k_iters = (f[i].a[0].cols + kK - 1) / kK;
     q.tiles_m = (q.M + 255) / 256;
     q.tiles_n = (q.N + bn - 1) / bn;
-    // a sum that is longer than a pair's share is shared out, eight stages or more to a pair
-    const long all = (long)q.k_iters * q.npairs, least = share > 8 ? share : 8;
-    long splits = (all + least / 2) / least;
-    if (splits > 64) splits = 64;
-    q.splits = splits < 1 ? 1 : (int)splits;
+    q.splits = splits[f[i].trans];
     const long n = (long)q.tiles_m * q.tiles_n * q.nout * q.splits;
     items += n;
     if (items > 0x3fffffffL) return ERROR_UNSUPPORTED;
