@@ -429,13 +429,10 @@ int gated_product_deriv(cudamat* deriv, cudamat* gate, cudamat* up, cudamat* gat
     return 0;
   }
   const bool biases = grad_gate_bias || grad_up_bias, weights = grad_gate_w || grad_up_w;
-  // On parts, or as four products of the matrices themselves (`dot`), which read large weights faster for few cases but take
-  // matrices that TMA cannot address behind copies.  Microseconds, parts / dot: 784 x 500, 100 cases 30 / 41; 1024 x 1024, 128 cases
-  // 40 / 58; 1024 x 4096, 64 cases 79 / 95; 2048 x 8192, 64 cases 196 / 149, 4096 cases 2491 / 2849.
-  const bool aligned = V % 4 == 0 && H % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device) &&
-                       on16(gate->data_device) && on16(up->data_device);
-  const bool few = aligned && !gate_planes && N < 128 && (long)V * H >= 1L << 22;
-  const bool large = (long)V * H * N >= 1L << 16 && !few;
+  // On parts, or as four products of the matrices themselves (`dot`), which for layers this small take one launch each and no scratch.
+  // (Beyond, parts are at least as fast, or 11 % slower where few cases meet large weights: 784 x 500, 100 cases 22 us and 42; 2048 x
+  // 8192, 8 cases 154 and 138, 256 cases 238 and 236, 4096 cases 2471 and 2777.  They need nothing that a capture does not allow.)
+  const bool large = (long)V * H * N >= 1L << 16;
   const bool tc = V > 0 && (weights || grad_mat) && gemm_path() != 2 && (large || gemm_path() == 1) && tma_available();
   const int cases = gated_deriv_cases(N), blocks = (N + cases - 1) / cases;
   const bool split_w = tc && grad_mat && !gate_planes;

@@ -495,3 +495,46 @@ def test_the_largest_number_there_is(cm):
     A, X = w.astype(np.float64), x.astype(np.float64)
     within(get(gm), A.T @ X, by_terms(A.T, X))
     assert np.array_equal(get(um), -get(gm))
+
+
+@pytest.mark.parametrize("shape", [(2048, 2048, 40), (2048, 2304, 9), (40, 30, 20), (300, 200, 100)])
+def test_derivatives_recorded_before_they_ever_ran(cm, shape):
+    """Two graphs of one stream, of layers large and small over few cases and many, recorded without a call before them and replayed on
+    streams that nobody orders: each gives what the calls give."""
+    V, H, N = shape
+    rng = np.random.default_rng(V + N)
+    torch.zeros(1, device="cuda")
+    sets, graphs, streams = [], [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in graphs:
+        r = lambda *s: cm.CUDAMatrix(rng.standard_normal(s).astype(np.float32))
+        sets.append(dict(w=(r(V, H), r(V, H)), x=r(V, N), dy=r(H, N), y=cm.empty((H, N)), gate=cm.empty((H, N)), up=cm.empty((H, N)),
+                         out=dict(grad_x=cm.empty((V, N)), grad_gate_w=cm.empty((V, H)), grad_up_w=cm.empty((V, H)), grad_up_bias=cm.empty((H, 1)))))
+
+    def step(s):
+        cm.gated_product(*s["w"], s["x"], s["y"], activation="silu", gate=s["gate"], up=s["up"])
+        cm.gated_product_deriv(s["dy"], s["gate"], s["up"], *s["w"], s["x"], activation="silu", **s["out"])
+    capture = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    cm._check(cm._lib.b200_set_stream(capture.cuda_stream))
+    try:
+        for s, graph in zip(sets, graphs):
+            with torch.cuda.graph(graph, stream=capture):
+                step(s)
+    finally:
+        cm._lib.b200_set_stream(None)
+    want = []
+    for s in sets:
+        step(s)
+        want.append([get(v) for v in [s["y"]] + list(s["out"].values())])
+        for v in [s["y"]] + list(s["out"].values()):
+            v.assign(0)
+    cm.cuda_sync_threads()
+    for _ in range(4):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for s, w in zip(sets, want):
+        for v, x in zip([s["y"]] + list(s["out"].values()), w):
+            assert np.array_equal(get(v), x)
+    assert cm.read_status() == 0
