@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 // Error codes of the reference C ABI (cudamat/cudamat.cuh:1-9) plus two new ones.
 #define ERROR_INCOMPATIBLE_DIMENSIONS -1
 #define CUBLAS_ERROR -2
@@ -99,6 +101,12 @@ inline cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 bl
 inline long numel(const cudamat* m) { return (long)m->size[0] * m->size[1]; }
 inline bool same_shape(const cudamat* a, const cudamat* b) {
   return a->size[0] == b->size[0] && a->size[1] == b->size[1];
+}
+// Whether something that is written lies over anything else (the error is set): the first `written` matrices may lie over none.
+bool overlapping(std::initializer_list<const cudamat*> mats, int written);
+// `mat`, or null where it is `result` itself, which a call may write in place.
+inline const cudamat* unless_in_place(const cudamat* mat, const cudamat* result) {
+  return mat && result && mat->data_device == result->data_device && same_shape(mat, result) ? nullptr : mat;
 }
 
 // ---------------------------------------------------------------- Philox4x32-10

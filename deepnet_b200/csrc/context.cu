@@ -218,6 +218,20 @@ void* workspace_zeroed(int slot, size_t bytes) {
   return p;
 }
 
+bool overlapping(std::initializer_list<const cudamat*> mats, int written) {
+  for (int i = 0; i < written; i++)
+    for (int j = i + 1; j < (int)mats.size(); j++) {
+      const cudamat *a = mats.begin()[i], *b = mats.begin()[j];
+      if (!a || !b || numel(a) == 0 || numel(b) == 0) continue;
+      const uintptr_t x = (uintptr_t)a->data_device, y = (uintptr_t)b->data_device;
+      if (x < y + 4 * numel(b) && y < x + 4 * numel(a)) {
+        set_error("a result may not lie over another argument");
+        return true;
+      }
+    }
+  return false;
+}
+
 CallScratch::CallScratch(int slot, size_t bytes) : p(nullptr), of_graph(false) {
   if (bytes == 0) return;
   if (!stream_capturing()) {

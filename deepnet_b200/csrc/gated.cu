@@ -2,8 +2,6 @@
 // and the derivative.  Weights are inputs x units, as an edge's; x is inputs x cases.
 //   G = Wg' x + bg,  U = Wu' x + bu,  y = act(G) U
 //   dU = dy act(G),  dG = dy U act'(G),  dx = Wg dG + Wu dU,  dWg = x dG',  dWu = x dU',  dbg, dbu: row sums of dG, dU
-#include <initializer_list>
-
 #include "gated.cuh"
 #include "gemm.cuh"
 
@@ -247,20 +245,6 @@ int weights_ok(const cudamat* gate_w, const cudamat* up_w) {
   if (!gate_w->on_device || !up_w->on_device) return ERROR_NOT_ON_DEVICE;
   if (gate_w->is_trans || up_w->is_trans) return ERROR_TRANSPOSED;
   return same_shape(gate_w, up_w) ? 0 : ERROR_INCOMPATIBLE_DIMENSIONS;
-}
-// Whether something that is written lies over anything else: the first `written` matrices may lie over none.
-bool overlapping(std::initializer_list<const cudamat*> mats, int written) {
-  for (int i = 0; i < written; i++)
-    for (int j = i + 1; j < (int)mats.size(); j++) {
-      const cudamat *a = mats.begin()[i], *b = mats.begin()[j];
-      if (!a || !b || numel(a) == 0 || numel(b) == 0) continue;
-      const uintptr_t x = (uintptr_t)a->data_device, y = (uintptr_t)b->data_device;
-      if (x < y + 4 * numel(b) && y < x + 4 * numel(a)) {
-        set_error("a result may not lie over another argument");
-        return true;
-      }
-    }
-  return false;
 }
 // Parts of both weights: all three matrices, on 16 bytes.
 int planes_ok(const cudamat* w, const cudamat* gate_planes, const cudamat* up_planes, const cudamat* low_planes) {

@@ -499,6 +499,7 @@ int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, cuda
     set_error("eps has to be at least 0");
     return ERROR_UNSUPPORTED;
   }
+  if (overlapping({target, stats, unless_in_place(mat, target), gain, bias}, 2)) return ERROR_UNSUPPORTED;
   if (h == 0 || w == 0) return 0;
   const float *x = mat->data_device, *g = gain ? gain->data_device : nullptr, *b = bias ? bias->data_device : nullptr;
   float *y = target->data_device, *st = stats ? stats->data_device : nullptr;
@@ -554,6 +555,10 @@ int layer_norm_deriv(cudamat* deriv, cudamat* mat, cudamat* stats, cudamat* gain
   if (!err) err = vector_ok(grad_gain, h);
   if (!err) err = vector_ok(grad_bias, h);
   if (err) return err;
+  // (the parameters' gradients are written when gain has been read)
+  if (overlapping({target, grad_gain, grad_bias, unless_in_place(deriv, target), unless_in_place(mat, target), stats,
+                   unless_in_place(unless_in_place(gain, grad_gain), grad_bias)}, 3))
+    return ERROR_UNSUPPORTED;
   if (h == 0) return 0;
   float *dgain = grad_gain ? grad_gain->data_device : nullptr, *dbias = grad_bias ? grad_bias->data_device : nullptr;
   if (w == 0) {            // sums over no columns

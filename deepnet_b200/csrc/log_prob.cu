@@ -417,6 +417,7 @@ int log_prob(cudamat* logits, cudamat* tokens, cudamat* target, cudamat* entropy
   if ((stats && (stats->size[0] != 2 || stats->size[1] != w)) || !top != !top_tokens ||
       (top && (!same_shape(top, top_tokens) || top->size[1] != w || top->size[0] > h)) || !tokens != !target)
     return ERROR_INCOMPATIBLE_DIMENSIONS;
+  if (overlapping({target, entropy, stats, top, top_tokens, logits, unless_in_place(tokens, target)}, 5)) return ERROR_UNSUPPORTED;
   if (w == 0) return 0;
   if (h == 0 || h > (1 << 24) || (top && top->size[0] > kMostTop)) {
     set_error(h == 0 ? "columns without a logit have no distribution"
@@ -456,6 +457,7 @@ int log_prob_deriv(cudamat* logits, cudamat* tokens, cudamat* stats, cudamat* gr
   if (err) return err;
   if (!same_shape(logits, target) || stats->size[0] != 2 || stats->size[1] != w || (grad && !tokens) || (grad_entropy && !entropy))
     return ERROR_INCOMPATIBLE_DIMENSIONS;
+  if (overlapping({target, unless_in_place(logits, target), tokens, stats, grad, entropy, grad_entropy}, 1)) return ERROR_UNSUPPORTED;
   if (h == 0 || w == 0) return 0;
   if (h > (1 << 24)) {
     set_error("a float32 does not hold every token of a column");

@@ -143,6 +143,7 @@ int dropout_scaled(rnd_struct* rnd_state, cudamat* mat, cudamat* add, cudamat* t
     set_error("the probability has to lie in 0 .. 1");
     return ERROR_UNSUPPORTED;
   }
+  if (overlapping({target, unless_in_place(mat, target), unless_in_place(add, target)}, 1)) return ERROR_UNSUPPORTED;
   const PhiloxKey key = make_philox_key(rnd_state->seed, rnd_state->calls);
   rnd_state->calls += 1;
   const int h = mat->size[0], w = mat->size[1], col0 = rng_col0();

@@ -293,6 +293,7 @@ int sample_multinomial(rnd_struct* rnd_state, cudamat* probs, cudamat* nn, cudam
 int add_sq_diff(cudamat* a, cudamat* b, cudamat* acc);
 
 /* ---- layers trained by gradients, words scored (no counterpart in the reference) ------ */
+/* Results lie over no other argument, in whole or in part, unless it says that they may. */
 /* Columns normalised: target = gain (x - mean) / sqrt(variance + eps) + bias, column by column; gain and bias (one value a row)
  * may be null, target may be mat.  stats (2 x columns, or null) receives mean and 1 / sqrt(variance + eps) for the derivative. */
 int layer_norm(cudamat* mat, cudamat* gain, cudamat* bias, cudamat* target, cudamat* stats, float eps);

@@ -171,3 +171,47 @@ def test_results_may_not_lie_over_other_arguments():
             m = {n: sq(p) for n, p in place.items()}
             assert cm._lib.gated_product_deriv(m["dy"], m["gate"], m["up"], m["wg"], m["wu"], m["x"], ct.c_int(1), None, None, None, m["dx"],
                                                m["dwg"], m["dwu"], None, None) == UNSUPPORTED, (a, b)
+
+
+def test_results_lie_over_an_argument_in_place_or_not_at_all():
+    """A byte in common is enough, but for the places that the documentation gives; what is refused draws nothing."""
+    lib, at = cm._lib, 1 << 30
+    h, w = 16, 8
+    x = lambda off=0, rows=h, cols=w: mat(rows, cols, at=at + off)
+    far = lambda rows=h, cols=w: mat(rows, cols)
+    for off in (4, -4, 4 * h, 4 * h * w - 4, 4 - 4 * h * w):
+        assert norm(x(), None, None, x(off), None) == UNSUPPORTED
+        assert lib.layer_norm_deriv(x(), far(), far(2), None, x(off), None, None) == UNSUPPORTED
+        assert lib.layer_norm_deriv(far(), x(), far(2), None, x(off), None, None) == UNSUPPORTED
+        assert lib.log_prob_deriv(x(), far(1), far(2), far(1), None, None, x(off)) == UNSUPPORTED
+        for m, add in ((x(), None), (far(), x())):
+            state = cm.rnd_struct(3, 7)
+            assert lib.dropout_scaled(ct.byref(state), m, add, x(off), ct.c_float(0.5)) == UNSUPPORTED and state.calls == 7
+    inside = 4 * (h * w - 1)
+    assert norm(x(), None, None, far(), x(inside, 2)) == UNSUPPORTED and norm(x(), None, None, x(), x(inside, 2)) == UNSUPPORTED
+    assert norm(far(), x(inside, h, 1), None, x(), None) == UNSUPPORTED and norm(far(), None, x(inside, 1, h), x(), None) == UNSUPPORTED
+    deriv = lambda *a: lib.layer_norm_deriv(*a)
+    assert deriv(far(), far(), x(inside, 2), None, x(), None, None) == UNSUPPORTED
+    assert deriv(far(), far(), far(2), x(inside, h, 1), x(), None, None) == UNSUPPORTED
+    assert deriv(x(), far(), far(2), None, far(), x(inside, h, 1), None) == UNSUPPORTED
+    assert deriv(far(), x(), far(2), None, far(), None, x(inside, h, 1)) == UNSUPPORTED
+    assert deriv(far(), far(), far(2), None, far(), x(0, h, 1), x(60, h, 1)) == UNSUPPORTED
+    assert deriv(far(), far(), far(2), x(0, h, 1), far(), x(4, h, 1), None) == UNSUPPORTED
+    row = lambda off: x(off, 1)
+    score = lambda z, t, *out: lib.log_prob(z, t, *out)
+    none = [None] * 5
+    for i, rows in enumerate((1, 1, 2, 3, 3)):
+        out = [far(1)] + none[1:]
+        out[i] = x(inside, rows)
+        if i > 2:
+            out[7 - i] = far(3)
+        assert score(x(), far(1), *out) == UNSUPPORTED
+        for j in range(i):
+            two = [far(1), far(1), far(2), far(3), far(3)]
+            two[i], two[j] = x(0, rows), x(4, (1, 1, 2, 3, 3)[j])
+            assert score(far(), far(1), *two) == UNSUPPORTED
+    assert score(far(), row(0), row(4), *none[1:]) == UNSUPPORTED
+    for i in range(5):
+        args = [far(1), far(2), far(1), far(1), far(1)]
+        args[i] = x(inside, 2 if i == 1 else 1)
+        assert lib.log_prob_deriv(far(), *args, x()) == UNSUPPORTED
