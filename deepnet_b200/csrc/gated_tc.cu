@@ -682,7 +682,9 @@ int plane_products(const PlaneProduct* f, int nproducts, int V, int H, int cases
   const long pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
   // The tile's width and how many each product's sums are shared out to (a pair of CTAs walks the items pairs apart, the inputs' gradient
   // first): what the pair with most work needs, in cycles, as in gated_tc.  As if all gradients were wanted, so that none's bits depend on
-  // the others.  Fitted to the same 20 shapes: 3 % above the best on average, 30 % at most (128 x 2000, 150 cases: 33 us, 26).
+  // the others.  Fitted to the same 20 shapes: 3 % above the best on average, 30 % at most (128 x 2000, 150 cases: 33 us, 26);
+  // the way through memory at twice its fitted price, as what it evens out does not pay where the power cap sets the clock (2048 x 8192,
+  // 4096 cases: shares of four 110 us in memory, the product no shorter).
   int bn = 256, splits[2] = {1, 1};
   double best = 0;
   for (int w = 256; w >= 128; w /= 2) {
@@ -702,7 +704,7 @@ int plane_products(const PlaneProduct* f, int nproducts, int V, int H, int cases
           const double t = c0 * l0 + (c - c0) * l1;
           if (t > cost) cost = t;
         }
-        if (s0 > 1 || s1 > 1) cost += 4200.0 + ((s0 > 1 ? (double)s0 * size[0] : 0.0) + (s1 > 1 ? (double)s1 * size[1] : 0.0)) / 300.0;
+        if (s0 > 1 || s1 > 1) cost += 4200.0 + ((s0 > 1 ? (double)s0 * size[0] : 0.0) + (s1 > 1 ? (double)s1 * size[1] : 0.0)) / 150.0;
         if (best == 0 || cost < best) {
           best = cost;
           bn = w;
