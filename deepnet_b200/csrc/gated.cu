@@ -329,7 +329,7 @@ int gated_product(cudamat* gate_w, cudamat* up_w, cudamat* mat, cudamat* gate_bi
   if (H == 0 || N == 0) return 0;
   if (overlapping({target, gate, up, mat, gate_w, up_w, gate_bias, up_bias, gate_planes, up_planes, low_planes}, 3)) return ERROR_UNSUPPORTED;
   auto at = [](cudamat* m) { return m ? m->data_device : nullptr; };
-  // Of large layers the tensor cores read planes faster from five cases on: 2048 x 8192, 8 cases 38 us, 51 without planes (123 with the
+  // Of large layers the tensor cores read planes faster from five cases on: 2048 x 8192, 8 cases 38 us, 50 without planes (94 with the
   // split before them), 5 cases 38 and 41, 4 cases 38 and 34.
   const bool on_groups = V % 4 == 0 && on16(gate_w->data_device) && on16(up_w->data_device) && on16(mat->data_device);
   const bool planes_first = gate_planes && N > 4 && (long)V * H >= 1L << 22;
